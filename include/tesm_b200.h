@@ -42,7 +42,8 @@ enum { TESM_LAYOUT_ROWMAJOR = 0, TESM_LAYOUT_GEMV = 1 };
 
 const char *tesm_b200_last_error(void);
 int tesm_b200_version(void);
-/* Reads and clears the sticky device status word (TESM_ETIMEOUT after a wait gave up). */
+/* Reads and clears the sticky device status word (TESM_ETIMEOUT after a wait gave up, TESM_EINVAL
+ * after tesm_b200_reorder_states met a parent out of range). */
 int tesm_b200_device_status(int *status_out);
 
 /* ---------------------------------------------------------------- BitLinear
@@ -329,6 +330,67 @@ int tesm_b200_siso_scan_noalloc(const void *proj, int dtype, int64_t ldp, int64_
                                 int64_t D, int64_t R, int64_t scan_chunk, const float *decay_bias,
                                 const double *h0, float *states, float *final_f32, double *final_f64,
                                 tesm_stream_t stream);
+
+/* ---------------------------------------------------------------- beam search
+ * One selection step.  logits (G prompts x W beams x V, unit stride over the vocabulary, element
+ * strides ldg / ldw), scores (G x W) the beams' summed log-probabilities.  A live beam w offers
+ * for every token v the score  scores[w] + logits[w,v] - logsumexp(logits[w])  at length
+ * lengths[w] + 1; a beam with finished[w] != 0 offers itself alone (token `pad`, its score and
+ * length unchanged; its logits are not read).  The K candidates with the largest
+ * score / max(length, 1)^length_penalty win, ties go to the lower beam, then the lower token.
+ * Candidates are formed and compared in fp64.  Outputs (G x K): tokens, parents (the beam
+ * a candidate continues), scores, finished (parent finished, or token == eos; pass eos = -1 for
+ * none), lengths.  Candidates of score -inf or NaN never win: a slot k that no candidate is left
+ * for gets parent min(k, W - 1), token pad, score -inf, finished.  A NaN logit counts as -inf, +inf
+ * as the largest finite float.  finished and lengths are nullable (none finished; lengths 0, only
+ * with length_penalty == 0).  1 <= W, K <= 32.  Two launches; ws: 16-byte aligned scratch of
+ * tesm_b200_beam_select_workspace bytes, free again once the work has run on the stream. */
+int tesm_b200_beam_select_workspace(int64_t G, int64_t W, int64_t V, int64_t K, int64_t *bytes_out);
+int tesm_b200_beam_select(const void *logits, int dtype, int64_t ldg, int64_t ldw, int64_t G, int64_t W, int64_t V,
+                          int64_t K, const float *scores, const uint8_t *finished, const int32_t *lengths,
+                          int64_t eos, int64_t pad, double length_penalty, int64_t *tokens, int32_t *parents,
+                          float *out_scores, uint8_t *out_finished, int32_t *out_lengths, void *ws, int64_t ws_bytes,
+                          tesm_stream_t stream);
+
+/* States follow their beams: row g * Wout + k of every dst becomes row g * Win + parents[g, k] of
+ * its src (bit copies; sizes and strides in bytes).  src == dst works in place (Win == Wout, equal
+ * strides); otherwise src and dst must not overlap, and no two entries may share memory.  `states`
+ * is a host array of n entries, read before the call returns; 128 entries go through one launch.
+ * A parent outside [0, Win) leaves its row as it is and sets the device status to
+ * TESM_EINVAL (tesm_b200_device_status).  1 <= Wout <= 32. */
+typedef struct {
+  const void *src;
+  void *dst;
+  int64_t row_bytes, src_stride, dst_stride;
+} tesm_b200_state_rows;
+int tesm_b200_reorder_states(const tesm_b200_state_rows *states, int64_t n, int64_t G, int64_t Win, int64_t Wout,
+                             const int32_t *parents, tesm_stream_t stream);
+
+/* ---------------------------------------------------------------- selective state space scan
+ * Short causal depthwise convolution, for prompts and (L = 1) single tokens:
+ *   out[b,t,d] = act(bias[d] + sum_j weight[d,j] * x[b, t-K+1+j, d]),  act = SiLU or identity,
+ * x and out (B, L, D) with unit channel stride and element strides ldxb / ldxl, ldob / ldol (out must not
+ * overlap x), weight (D, K) and bias (D, nullable) fp32, 2 <= K <= 8, fp32 accumulation.  state
+ * (B, K-1, D) of x's dtype, dense, nullable: the inputs before the first token (zeros without it),
+ * replaced by the last K - 1 inputs.  lengths (B, nullable): sequence b holds its first
+ * lengths[b] tokens; the outputs behind them are zeros, a length of 0 leaves the state as it is. */
+int tesm_b200_causal_conv(const void *x, int dtype, int64_t ldxb, int64_t ldxl, int64_t B, int64_t L, int64_t D,
+                          int64_t K, const float *weight, const float *bias, void *state, const int32_t *lengths,
+                          int silu, void *out, int64_t ldob, int64_t ldol, tesm_stream_t stream);
+
+/* Selective scan with N states per channel, for prompts and (L = 1) single tokens:
+ *   dt = softplus(dt_raw + dt_bias)  (or dt_raw + dt_bias with softplus == 0),
+ *   h[d,n] = exp(dt[d] A[d,n]) h[d,n] + dt[d] x[d] bm[n],   y[d] = sum_n cm[n] h[d,n] + skip[d] x[d],
+ *   out[d] = y[d] * silu(z[d])  (y[d] with z == NULL).
+ * x, dt, z, out (B, L, D) and bm, cm (B, L, N) of one dtype, unit innermost stride; strides: 12
+ * element strides (batch, token) of x, dt, bm, cm, z, out.  A (D, N), skip (D), dt_bias (D) fp32, the
+ * last two nullable.  state (B, D, N) fp32, dense, nullable: the state before the first token
+ * (zeros without it), replaced by the one after the last.  lengths as in tesm_b200_causal_conv.  out
+ * must not overlap the inputs.  1 <= N <= 128; states and sums in fp32. */
+int tesm_b200_ssm_scan(const void *x, const void *dt, const void *bm, const void *cm, const void *z, void *out,
+                       const int64_t *strides, int dtype, int64_t B, int64_t L, int64_t D, int64_t N, const float *A,
+                       const float *skip, const float *dt_bias, int softplus, float *state, const int32_t *lengths,
+                       tesm_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -19,6 +19,7 @@ _lib = None
 c_i64 = ctypes.c_int64
 c_int = ctypes.c_int
 c_float = ctypes.c_float
+c_double = ctypes.c_double
 c_vp = ctypes.c_void_p
 
 # name -> argument types (all return int status unless listed in _RESTYPES)
@@ -80,8 +81,21 @@ SIGNATURES = {
                                  c_vp, c_i64, c_vp],
     "tesm_b200_siso_scan_noalloc": [c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp,
                                     c_vp, c_vp, c_vp, c_vp],
+    "tesm_b200_beam_select_workspace": [c_i64, c_i64, c_i64, c_i64, c_vp],
+    "tesm_b200_beam_select": [c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_i64, c_i64,
+                              c_double, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp],
+    "tesm_b200_reorder_states": [c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp],
+    "tesm_b200_causal_conv": [c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_int,
+                              c_vp, c_i64, c_i64, c_vp],
+    "tesm_b200_ssm_scan": [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp,
+                           c_vp, c_int, c_vp, c_vp, c_vp],
 }
 _RESTYPES = {"tesm_b200_last_error": ctypes.c_char_p}
+
+
+class StateRows(ctypes.Structure):
+    """tesm_b200_state_rows of the C header."""
+    _fields_ = [("src", c_vp), ("dst", c_vp), ("row_bytes", c_i64), ("src_stride", c_i64), ("dst_stride", c_i64)]
 
 
 class TesmError(RuntimeError):
@@ -122,7 +136,8 @@ def check(status: int, what: str):
 
 # number of entry-point calls that enqueue device work (bench.py reports it as gpu_launches)
 launch_count = 0
-_NO_LAUNCH = {"tesm_b200_version", "tesm_b200_last_error", "tesm_b200_device_status", "tesm_b200_scan_workspace"}
+_NO_LAUNCH = {"tesm_b200_version", "tesm_b200_last_error", "tesm_b200_device_status", "tesm_b200_scan_workspace",
+              "tesm_b200_beam_select_workspace"}
 
 
 def call(name: str, *args):

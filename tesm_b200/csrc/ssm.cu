@@ -1,0 +1,535 @@
+// Selective state space scan and the short causal convolution in front of it, for prompts and for
+// single tokens.
+#include "common.cuh"
+
+namespace tesm {
+
+// x * sigmoid(x); 0 for x -> -inf (the reciprocal of inf is 0, and x * 0 stays finite for finite x)
+__device__ __forceinline__ float silu(float x) { return x * rcp_approx(1.f + ex2_approx(-x * kLog2e)); }
+
+// softplus(x) = max(x, 0) + log(1 + u), u = e^-|x| in (0, 1].  log(1 + u) = 2 atanh(s) with
+// s = u / (2 + u) <= 1/3: the odd series in s keeps full relative accuracy for small u, where
+// forming 1 + u would round u away.  Terms to s^15 leave 1.4e-9 relative at s = 1/3.
+__device__ __forceinline__ float softplus(float x) {
+  const float u = ex2_approx(-fabsf(x) * kLog2e);
+  const float s = u * rcp_approx(2.f + u), q = s * s;
+  float p = 1.f / 15.f;
+  p = fmaf(p, q, 1.f / 13.f);
+  p = fmaf(p, q, 1.f / 11.f);
+  p = fmaf(p, q, 1.f / 9.f);
+  p = fmaf(p, q, 1.f / 7.f);
+  p = fmaf(p, q, 1.f / 5.f);
+  p = fmaf(p, q, 1.f / 3.f);
+  p = fmaf(p, q, 1.f);
+  return fmaxf(x, 0.f) + 2.f * s * p;
+}
+
+template <class T>
+__device__ __forceinline__ float to_f(T x);
+template <>
+__device__ __forceinline__ float to_f(float x) { return x; }
+template <>
+__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <class T>
+__device__ __forceinline__ T from_f(float x);
+template <>
+__device__ __forceinline__ float from_f(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f(float x) { return __float2bfloat16_rn(x); }
+
+// N consecutive elements as they are in memory: one 16-byte access per 16 bytes where `vec`
+// promises alignment and all N exist, else the first `have` of them one by one (the rest zero).
+template <class T, int N>
+struct Pack {
+  T v[N];
+  __device__ __forceinline__ void load(const T *p, bool vec, int have) {
+    if constexpr (N * sizeof(T) % 16 == 0) {
+      if (vec && have >= N) {
+#pragma unroll
+        for (int i = 0; i < (int)(N * sizeof(T) / 16); ++i)
+          reinterpret_cast<uint4 *>(v)[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+        return;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = i < have ? p[i] : from_f<T>(0.f);
+  }
+  __device__ __forceinline__ void store(T *p, bool vec, int have) const {
+    if constexpr (N * sizeof(T) % 16 == 0) {
+      if (vec && have >= N) {
+#pragma unroll
+        for (int i = 0; i < (int)(N * sizeof(T) / 16); ++i)
+          reinterpret_cast<uint4 *>(p)[i] = reinterpret_cast<const uint4 *>(v)[i];
+        return;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < have) p[i] = v[i];
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = from_f<T>(0.f);
+  }
+};
+
+// A (batch, token, channel) tensor with unit channel stride.
+template <class T>
+struct Rows {
+  T *p;
+  int64_t ldb, ldl;
+  __device__ __forceinline__ T *at(int64_t b, int64_t t, int64_t c) const { return p + b * ldb + t * ldl + c; }
+};
+
+__device__ __forceinline__ int seq_len(const int *lengths, int64_t b, int L) {
+  return lengths ? min(max(lengths[b], 0), L) : L;
+}
+
+// ------------------------------------------------------------ causal convolution
+// y_t = act(bias + sum_j w_j x_{t-K+1+j}).  A thread owns N channels (16 bytes of them) and walks
+// a tile of tokens with the last K - 1 inputs in registers, so x is read once (and K - 1 rows
+// again per tile) and y written once.
+constexpr int kConvThreads = 128;
+
+template <class T, int N, int K>
+__global__ void __launch_bounds__(kConvThreads)
+    k_causal_conv(Rows<const T> x, int L, int D, int TT, int vec, const float *__restrict__ weight,
+                  const float *__restrict__ bias, T *__restrict__ state, const int *__restrict__ lengths, int act,
+                  Rows<T> y, int chunks, int tiles) {
+  pdl_trigger();
+  pdl_wait();
+  const int chunk = blockIdx.x % chunks;
+  const int tile = blockIdx.x / chunks % tiles;
+  const int64_t b = blockIdx.x / chunks / tiles;
+  const int c = (chunk * kConvThreads + threadIdx.x) * N;
+  if (c >= D) return;
+  const int have = min(N, D - c);
+  const int T_b = seq_len(lengths, b, L);
+  T *st = state ? state + (b * (K - 1)) * D + c : nullptr;
+  // the input of position p >= 1 - K; before the start the state's rows
+  auto load = [&](Pack<T, N> &q, int p) {
+    if (p >= 0)
+      q.load(x.at(b, p, c), vec, have);
+    else if (st)
+      q.load(st + (int64_t)(p + K - 1) * D, vec, have);
+    else
+      q.zero();
+  };
+  const int t0 = tile * TT, t1 = min(t0 + TT, L), te = min(t1, T_b);
+  if (t0 < te) {
+    float w[K][N], bs[N], win[K][N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      bs[e] = bias && e < have ? bias[c + e] : 0.f;
+#pragma unroll
+      for (int j = 0; j < K; ++j) w[j][e] = e < have ? weight[(int64_t)(c + e) * K + j] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j) {
+      Pack<T, N> q;
+      load(q, t0 - (K - 1) + j);
+#pragma unroll
+      for (int e = 0; e < N; ++e) win[j][e] = to_f(q.v[e]);
+    }
+    constexpr int U = 4;  // rows loaded ahead of their use
+    for (int t = t0; t < te; t += U) {
+      Pack<T, N> in[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (t + u < te) in[u].load(x.at(b, t + u, c), vec, have);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (t + u >= te) break;
+        Pack<T, N> out;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          win[K - 1][e] = to_f(in[u].v[e]);
+          float acc = bs[e];
+#pragma unroll
+          for (int j = 0; j < K; ++j) acc = fmaf(w[j][e], win[j][e], acc);
+          out.v[e] = from_f<T>(act ? silu(acc) : acc);
+#pragma unroll
+          for (int j = 0; j < K - 1; ++j) win[j][e] = win[j + 1][e];
+        }
+        out.store(y.at(b, t + u, c), vec, have);
+      }
+    }
+  }
+  Pack<T, N> z;
+  z.zero();
+  for (int t = max(t0, te); t < t1; ++t) z.store(y.at(b, t, c), vec, have);
+  // only the first tile reads the state, so the thread that has read it may replace it
+  if (tile == 0 && st && T_b > 0) {
+    Pack<T, N> q[K - 1];
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j) load(q[j], T_b - (K - 1) + j);
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j) q[j].store(st + (int64_t)j * D, vec, have);
+  }
+}
+
+// ------------------------------------------------------------ selective scan, prompts
+// h_t = exp(dt_t A) h_{t-1} + (dt_t x_t) B_t,  y_t = C_t . h_t + D x_t,  out = y silu(z).
+// A channel's N states are spread over LPC lanes with NPT states each (zero-padded to NPT * LPC);
+// a block of 128 threads walks the sequence of 128 / LPC channels in tiles of TT tokens.  Per
+// tile: softplus and dt * x are formed once per (token, channel) and staged in fp32 with B and
+// C; the raw rows of the next tile are loaded while this one is computed.  The sums over a
+// channel's lanes are transposed-reduced: LPC tokens' partial sums exchange halves in log2(LPC)
+// rounds, so that a token costs one shuffle instead of log2(LPC).
+constexpr int kScanThreads = 128;
+
+template <int NPT, int LPC>
+struct ScanShape {
+  static constexpr int NP = NPT * LPC;             // padded states per channel
+  static constexpr int CT = kScanThreads / LPC;    // channels per block
+  static constexpr int TT = LPC >= 32 ? 32 : LPC >= 8 ? 64 : 1024 / CT;  // tokens per tile
+  static constexpr int V = CT >= 8 ? 8 : 4;        // channels per row access
+  static constexpr int ITEMS = TT * CT / V;        // row accesses per tile and tensor (<= threads)
+  static constexpr int BV = NP >= 8 ? 8 : NP;      // states per access of B and C
+  static constexpr int BITEMS = TT * (NP / BV);
+  static constexpr int BIPT = (BITEMS + kScanThreads - 1) / kScanThreads;
+  static constexpr int SMEM = (TT * CT * 3 + 2 * TT * NP) * 4;
+};
+
+template <class T>
+struct ScanArgs {
+  Rows<const T> x, dt, bm, cm, z;
+  Rows<T> out;
+  const float *A, *skip, *dt_bias;
+  float *state;
+  const int *lengths;
+  int L, D, N, softplus, vec_rows, vec_bc, chunks;
+};
+
+template <class T, int NPT, int LPC>
+__global__ void __launch_bounds__(kScanThreads) k_ssm_scan(const __grid_constant__ ScanArgs<T> a) {
+  using S = ScanShape<NPT, LPC>;
+  constexpr int NP = S::NP, CT = S::CT, TT = S::TT, V = S::V, BV = S::BV, BIPT = S::BIPT;
+  static_assert(S::ITEMS <= kScanThreads && TT % LPC == 0, "one row access per thread and tile");
+  extern __shared__ __align__(16) float smem[];
+  float2 *su = reinterpret_cast<float2 *>(smem);  // [TT][CT] {dt, dt * x}
+  float *sb = smem + 2 * TT * CT;                 // [TT][NP]
+  float *sc = sb + TT * NP;
+  float *sy = sc + TT * NP;                       // [TT][CT]
+  pdl_trigger();
+  pdl_wait();
+  const int tid = threadIdx.x;
+  const int64_t b = blockIdx.x / a.chunks;
+  const int c0 = (int)(blockIdx.x % a.chunks) * CT;
+  const int T_b = seq_len(a.lengths, b, a.L);
+  const int tiles = (T_b + TT - 1) / TT;
+
+  // the states of this thread
+  const int ch = tid / LPC, q = tid % LPC, n0 = q * NPT;
+  const bool live = c0 + ch < a.D;
+  float A2[NPT], h[NPT];
+#pragma unroll
+  for (int i = 0; i < NPT; ++i) {
+    const int64_t at = (int64_t)(c0 + ch) * a.N + n0 + i;
+    const bool on = live && n0 + i < a.N;
+    A2[i] = on ? a.A[at] * kLog2e : 0.f;
+    h[i] = on && a.state ? a.state[b * (int64_t)a.D * a.N + at] : 0.f;
+  }
+
+  // the row access of this thread: token rt of a tile, channels c0 + rc ...
+  const bool loads = tid < S::ITEMS;
+  const int rt = tid / (CT / V), rc = tid % (CT / V) * V;
+  const int have = loads ? min(V, a.D - c0 - rc) : 0;  // may be <= 0 behind the last channel
+  float bias[V], skip[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    bias[e] = e < have && a.dt_bias ? a.dt_bias[c0 + rc + e] : 0.f;
+    skip[e] = e < have && a.skip ? a.skip[c0 + rc + e] : 0.f;
+  }
+  Pack<T, V> nx, nd, nz;
+  Pack<T, BV> nb[BIPT], nc[BIPT];
+  auto fetch = [&](int tile) {
+    const int t = tile * TT + rt;
+    const int h_ = t < T_b ? have : 0;
+    nx.load(a.x.at(b, t, c0 + rc), a.vec_rows, h_);
+    nd.load(a.dt.at(b, t, c0 + rc), a.vec_rows, h_);
+    if (a.z.p) nz.load(a.z.at(b, t, c0 + rc), a.vec_rows, h_);
+#pragma unroll
+    for (int i = 0; i < BIPT; ++i) {
+      const int it = tid + i * kScanThreads, bt = it / (NP / BV), bn = it % (NP / BV) * BV;
+      const int t2 = tile * TT + bt;
+      const int hb = it < S::BITEMS && t2 < T_b ? a.N - bn : 0;
+      nb[i].load(a.bm.at(b, t2, bn), a.vec_bc, hb);
+      nc[i].load(a.cm.at(b, t2, bn), a.vec_bc, hb);
+    }
+  };
+  fetch(0);
+  for (int tile = 0; tile < tiles; ++tile) {
+    const Pack<T, V> x = nx, z = nz;
+    const bool tok = tile * TT + rt < T_b;
+    if (loads) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        float d = to_f(nd.v[e]) + bias[e];
+        if (a.softplus) d = softplus(d);
+        if (!tok) d = 0.f;  // behind the end: a = 1, no input
+        su[rt * CT + rc + e] = make_float2(d, d * to_f(x.v[e]));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < BIPT; ++i) {
+      const int it = tid + i * kScanThreads, at = it / (NP / BV) * NP + it % (NP / BV) * BV;
+      if (it < S::BITEMS) {
+#pragma unroll
+        for (int e = 0; e < BV; ++e) sb[at + e] = to_f(nb[i].v[e]), sc[at + e] = to_f(nc[i].v[e]);
+      }
+    }
+    __syncthreads();
+    if (tile + 1 < tiles) fetch(tile + 1);
+#pragma unroll 1
+    for (int t = 0; t < TT; t += LPC) {
+      float p[LPC];
+#pragma unroll
+      for (int j = 0; j < LPC; ++j) {
+        const float2 u = su[(t + j) * CT + ch];
+        const float *bp = sb + (t + j) * NP + n0, *cp = sc + (t + j) * NP + n0;
+        float acc = 0.f;
+#pragma unroll
+        for (int i = 0; i < NPT; ++i) {
+          h[i] = fmaf(ex2_approx(u.x * A2[i]), h[i], u.y * bp[i]);
+          acc = fmaf(cp[i], h[i], acc);
+        }
+        p[j] = acc;
+      }
+#pragma unroll
+      for (int o = LPC / 2; o; o >>= 1) {
+        const bool up = q & o;
+#pragma unroll
+        for (int j = 0; j < o; ++j) {
+          const float keep = up ? p[j + o] : p[j], give = up ? p[j] : p[j + o];
+          p[j] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+        }
+      }
+      sy[(t + q) * CT + ch] = p[0];  // lane q holds token t + q
+    }
+    __syncthreads();
+    if (loads && tok) {
+      Pack<T, V> o;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        float y = fmaf(skip[e], to_f(x.v[e]), sy[rt * CT + rc + e]);
+        if (a.z.p) y *= silu(to_f(z.v[e]));
+        o.v[e] = from_f<T>(y);
+      }
+      o.store(a.out.at(b, tile * TT + rt, c0 + rc), a.vec_rows, have);
+    }
+  }
+  // outputs behind the end are zeros
+  if (loads) {
+    Pack<T, V> o;
+    o.zero();
+    for (int t = T_b + rt; t < a.L; t += TT) o.store(a.out.at(b, t, c0 + rc), a.vec_rows, have);
+  }
+  if (a.state && live && T_b > 0) {
+#pragma unroll
+    for (int i = 0; i < NPT; ++i)
+      if (n0 + i < a.N) a.state[(b * a.D + c0 + ch) * (int64_t)a.N + n0 + i] = h[i];
+  }
+}
+
+// ------------------------------------------------------------ selective scan, single tokens
+// One token per sequence: the state is read and written once, which bounds it.  LPC lanes of 4
+// states per channel; a thread keeps its row of A for kStepBatch sequences.
+constexpr int kStepThreads = 256, kStepBatch = 8;
+
+template <class T, bool VEC>
+__global__ void __launch_bounds__(kStepThreads)
+    k_ssm_step(const __grid_constant__ ScanArgs<T> a, int B, int lpc) {
+  pdl_trigger();
+  pdl_wait();
+  const int per = kStepThreads / lpc;
+  const int q = threadIdx.x % lpc, n0 = q * 4;
+  const int c = (int)(blockIdx.x % a.chunks) * per + threadIdx.x / lpc;
+  const int b0 = (int)(blockIdx.x / a.chunks) * kStepBatch, b1 = min(b0 + kStepBatch, B);
+  const bool live = c < a.D;
+  const int have = live ? min(4, a.N - n0) : 0;
+  Pack<float, 4> A;
+  A.load(a.A + (int64_t)c * a.N + n0, VEC, have);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) A.v[i] *= kLog2e;
+  const float bias = live && a.dt_bias ? a.dt_bias[c] : 0.f, skip = live && a.skip ? a.skip[c] : 0.f;
+#pragma unroll 2
+  for (int b = b0; b < b1; ++b) {
+    const bool on = live && seq_len(a.lengths, b, 1) > 0;
+    const int hv = on ? have : 0;
+    Pack<float, 4> h;
+    h.zero();
+    float *st = a.state ? a.state + ((int64_t)b * a.D + c) * a.N + n0 : nullptr;
+    if (st) h.load(st, VEC, hv);
+    Pack<T, 4> bm, cm;
+    bm.load(a.bm.at(b, 0, n0), false, hv);
+    cm.load(a.cm.at(b, 0, n0), false, hv);
+    const float x = on ? to_f(*a.x.at(b, 0, c)) : 0.f;
+    float d = on ? to_f(*a.dt.at(b, 0, c)) + bias : 0.f;
+    if (a.softplus) d = softplus(d);
+    float y = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      h.v[i] = fmaf(ex2_approx(d * A.v[i]), h.v[i], d * x * to_f(bm.v[i]));
+      y = fmaf(to_f(cm.v[i]), h.v[i], y);
+    }
+    if (st) h.store(st, VEC, hv);
+    for (int o = lpc / 2; o; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+    if (q == 0 && live) {
+      y = fmaf(skip, x, y);
+      if (a.z.p && on) y *= silu(to_f(*a.z.at(b, 0, c)));
+      *a.out.at(b, 0, c) = from_f<T>(on ? y : 0.f);
+    }
+  }
+}
+
+template <class T, int NPT, int LPC>
+static int launch_scan(ScanArgs<T> a, int64_t B, cudaStream_t st) {
+  using S = ScanShape<NPT, LPC>;
+  if constexpr (S::SMEM > 48 * 1024) {
+    cudaError_t e = cudaFuncSetAttribute(k_ssm_scan<T, NPT, LPC>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    if (e != cudaSuccess) return fail(TESM_ELAUNCH, std::string("ssm_scan: ") + cudaGetErrorString(e));
+  }
+  a.chunks = (int)ceil_div(a.D, S::CT);
+  return launch_k("ssm_scan", k_ssm_scan<T, NPT, LPC>, dim3((unsigned)(B * a.chunks)), dim3(kScanThreads), S::SMEM, st,
+                  a);
+}
+
+template <class T, int NPT>
+static int launch_scan_lanes(const ScanArgs<T> &a, int64_t B, int lpc, cudaStream_t st) {
+  switch (lpc) {
+    case 1: return launch_scan<T, NPT, 1>(a, B, st);
+    case 2: return launch_scan<T, NPT, 2>(a, B, st);
+    case 4: return launch_scan<T, NPT, 4>(a, B, st);
+    case 8: return launch_scan<T, NPT, 8>(a, B, st);
+    case 16: return launch_scan<T, NPT, 16>(a, B, st);
+    default: return launch_scan<T, NPT, 32>(a, B, st);
+  }
+}
+
+template <class T>
+static int ssm_scan_t(ScanArgs<T> a, int64_t B, cudaStream_t st) {
+  int np = 1;
+  while (np < a.N) np <<= 1;
+  if (a.L == 1) {
+    const int lpc = np <= 4 ? 1 : np / 4;
+    a.chunks = (int)ceil_div(a.D, kStepThreads / lpc);
+    const dim3 grid((unsigned)(a.chunks * ceil_div(B, kStepBatch))), block(kStepThreads);
+    const bool vec = a.N % 4 == 0 && (((uintptr_t)a.A | (uintptr_t)a.state) & 15) == 0;
+    return vec ? launch_k("ssm_scan", k_ssm_step<T, true>, grid, block, 0, st, a, (int)B, lpc)
+               : launch_k("ssm_scan", k_ssm_step<T, false>, grid, block, 0, st, a, (int)B, lpc);
+  }
+  // States per lane: as many as still give every SM a block; fewer states per lane spread a
+  // channel over more lanes.
+  int npt = np >= 4 ? 4 : np;
+  while (npt > 1 && np / (npt / 2) <= 32 && B * ceil_div((int64_t)a.D * (np / npt), kScanThreads) < sm_count()) npt >>= 1;
+  const int lpc = np / npt;
+  return npt == 4   ? launch_scan_lanes<T, 4>(a, B, lpc, st)
+         : npt == 2 ? launch_scan_lanes<T, 2>(a, B, lpc, st)
+                    : launch_scan_lanes<T, 1>(a, B, lpc, st);
+}
+
+template <class T, int N>
+static int launch_conv(Rows<const T> x, int64_t B, int L, int D, int K, int vec, const float *w, const float *bias,
+                       T *state, const int *lengths, int act, Rows<T> y, cudaStream_t st) {
+  const int chunks = (int)ceil_div(D, kConvThreads * N);
+  int TT = 64;  // tokens per tile: shorter while the blocks do not fill the SMs
+  while (TT > 8 && B * chunks * ceil_div(L, TT) < 8 * (int64_t)sm_count()) TT >>= 1;
+  const int tiles = (int)ceil_div(L, TT);
+  const dim3 grid((unsigned)(B * chunks * tiles)), block(kConvThreads);
+#define TESM_CONV(KK)                                                                                            \
+  case KK:                                                                                                       \
+    return launch_k("causal_conv", k_causal_conv<T, N, KK>, grid, block, 0, st, x, L, D, TT, vec, w, bias, state, \
+                    lengths, act, y, chunks, tiles)
+  switch (K) {
+    TESM_CONV(2);
+    TESM_CONV(3);
+    TESM_CONV(4);
+    TESM_CONV(5);
+    TESM_CONV(6);
+    TESM_CONV(7);
+    TESM_CONV(8);
+  }
+#undef TESM_CONV
+  return fail(TESM_EUNSUPPORTED, "causal_conv: kernel width");
+}
+
+template <class T>
+static int causal_conv_t(const void *x, int64_t ldb, int64_t ldl, int64_t B, int64_t L, int64_t D, int64_t K,
+                         const float *w, const float *bias, void *state, const int *lengths, int act, void *y,
+                         int64_t ldyb, int64_t ldyl, cudaStream_t st) {
+  const Rows<const T> rx{(const T *)x, ldb, ldl};
+  const Rows<T> ry{(T *)y, ldyb, ldyl};
+  const uint64_t bits = (uintptr_t)x | (uintptr_t)y | (uintptr_t)state |
+                        (uint64_t)((ldb | ldl | ldyb | ldyl | (state ? D : 0)) * (int64_t)sizeof(T));
+  constexpr int N = 16 / sizeof(T);
+  if (bits % 16 == 0)
+    return launch_conv<T, N>(rx, B, (int)L, (int)D, (int)K, 1, w, bias, (T *)state, lengths, act, ry, st);
+  return launch_conv<T, 1>(rx, B, (int)L, (int)D, (int)K, 0, w, bias, (T *)state, lengths, act, ry, st);
+}
+
+}  // namespace tesm
+
+extern "C" int tesm_b200_causal_conv(const void *x, int dtype, int64_t ldxb, int64_t ldxl, int64_t B, int64_t L,
+                                     int64_t D, int64_t K, const float *weight, const float *bias, void *state,
+                                     const int32_t *lengths, int silu, void *out, int64_t ldob, int64_t ldol,
+                                     tesm_stream_t stream) {
+  using namespace tesm;
+  if (dtype != TESM_F32 && dtype != TESM_BF16) return fail(TESM_EDTYPE, "causal_conv: dtype");
+  TESM_REQUIRE(B >= 0 && L >= 0 && D >= 0 && L < (1ll << 30) && D < (1ll << 30), "causal_conv: bad shape");
+  if (K < 2 || K > 8) return fail(TESM_EUNSUPPORTED, "causal_conv: kernel width 2 to 8");
+  if (B == 0 || L == 0 || D == 0) return TESM_OK;
+  TESM_REQUIRE(x && weight && out, "causal_conv: null pointer");
+  TESM_REQUIRE(B * ceil_div(D, kConvThreads) * ceil_div(L, 8) < (1ll << 31), "causal_conv: too many blocks");
+  cudaStream_t st = (cudaStream_t)stream;
+  return dtype == TESM_BF16 ? causal_conv_t<__nv_bfloat16>(x, ldxb, ldxl, B, L, D, K, weight, bias, state, lengths, silu,
+                                                           out, ldob, ldol, st)
+                            : causal_conv_t<float>(x, ldxb, ldxl, B, L, D, K, weight, bias, state, lengths, silu, out,
+                                                   ldob, ldol, st);
+}
+
+namespace tesm {
+template <class T>
+static int ssm_scan_c(const void *x, const void *dt, const void *bm, const void *cm, const void *z, void *out,
+                      const int64_t *ld, int64_t B, ScanArgs<T> a, cudaStream_t st) {
+  a.x = {(const T *)x, ld[0], ld[1]};
+  a.dt = {(const T *)dt, ld[2], ld[3]};
+  a.bm = {(const T *)bm, ld[4], ld[5]};
+  a.cm = {(const T *)cm, ld[6], ld[7]};
+  a.z = {(const T *)z, ld[8], ld[9]};
+  a.out = {(T *)out, ld[10], ld[11]};
+  uint64_t rows = (uintptr_t)x | (uintptr_t)dt | (uintptr_t)z | (uintptr_t)out;
+  const int64_t es = sizeof(T);
+  for (int i : {0, 1, 2, 3, 10, 11}) rows |= (uint64_t)(ld[i] * es);
+  if (z) rows |= (uint64_t)(ld[8] * es) | (uint64_t)(ld[9] * es);
+  uint64_t bc = (uintptr_t)bm | (uintptr_t)cm;
+  for (int i : {4, 5, 6, 7}) bc |= (uint64_t)(ld[i] * es);
+  a.vec_rows = rows % 16 == 0;
+  a.vec_bc = bc % 16 == 0;
+  return ssm_scan_t<T>(a, B, st);
+}
+}  // namespace tesm
+
+extern "C" int tesm_b200_ssm_scan(const void *x, const void *dt, const void *bm, const void *cm, const void *z,
+                                  void *out, const int64_t *strides, int dtype, int64_t B, int64_t L, int64_t D,
+                                  int64_t N, const float *A, const float *skip, const float *dt_bias, int softplus,
+                                  float *state, const int32_t *lengths, tesm_stream_t stream) {
+  using namespace tesm;
+  if (dtype != TESM_F32 && dtype != TESM_BF16) return fail(TESM_EDTYPE, "ssm_scan: dtype");
+  TESM_REQUIRE(B >= 0 && L >= 0 && D >= 0 && L < (1ll << 30) && D < (1ll << 30), "ssm_scan: bad shape");
+  if (N < 1 || N > 128) return fail(TESM_EUNSUPPORTED, "ssm_scan: 1 to 128 states per channel");
+  if (B == 0 || L == 0 || D == 0) return TESM_OK;
+  TESM_REQUIRE(x && dt && bm && cm && out && A && strides, "ssm_scan: null pointer");
+  TESM_REQUIRE(B * ceil_div(D, 4) < (1ll << 31), "ssm_scan: too many blocks");
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == TESM_BF16) {
+    ScanArgs<__nv_bfloat16> a = {};
+    a.A = A, a.skip = skip, a.dt_bias = dt_bias, a.state = state, a.lengths = lengths;
+    a.L = (int)L, a.D = (int)D, a.N = (int)N, a.softplus = softplus;
+    return ssm_scan_c<__nv_bfloat16>(x, dt, bm, cm, z, out, strides, B, a, st);
+  }
+  ScanArgs<float> a = {};
+  a.A = A, a.skip = skip, a.dt_bias = dt_bias, a.state = state, a.lengths = lengths;
+  a.L = (int)L, a.D = (int)D, a.N = (int)N, a.softplus = softplus;
+  return ssm_scan_c<float>(x, dt, bm, cm, z, out, strides, B, a, st);
+}

@@ -9,7 +9,8 @@ from __future__ import annotations
 import ctypes
 import os
 from dataclasses import dataclass
-from typing import Optional
+from functools import lru_cache
+from typing import Optional, Sequence
 
 import torch
 
@@ -502,3 +503,289 @@ def mimo_global_ent(proj, B, L, Dm, H, D, R, RM, relb, mimo_o, states, thr, base
     _lib.call("tesm_b200_mimo_global_ent", proj.data_ptr(), dtype_code(proj.dtype), proj.stride(0), B, L, Dm, H, D,
               R, RM, relb.data_ptr(), mimo_o.data_ptr(), states.data_ptr(), float(thr), float(base), _ptr(acc_e),
               _ptr(acc_c), out_tanh.data_ptr(), out_chg.data_ptr(), dtype_code(out_tanh.dtype), _stream())
+
+
+# ------------------------------------------------------------------ beam search
+MAX_BEAMS = 32
+
+
+def _need(ok, what: str):
+    if not ok:
+        raise ValueError("tesm_b200 " + what)
+
+
+def _no_grad(what: str, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"tesm_b200 {what} has no autograd path (use torch.no_grad())")
+
+
+def _call_on(dev: torch.device, name: str, *args):
+    """Launch on ``dev``'s current stream, whichever device is current."""
+    if dev.index == torch.cuda.current_device():
+        _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+
+
+def _check(what: str, name: str, t: Optional[torch.Tensor], shape, dtype: torch.dtype, dev: torch.device):
+    """A dense tensor of this shape, type and device (or None)."""
+    if t is None:
+        return
+    _need(t.shape == shape and t.dtype == dtype and t.device == dev and t.is_contiguous(),
+          f"{what}: {name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {dev}, got "
+          f"{t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+@dataclass
+class BeamStep:
+    """One selection step: (prompts, beams) tensors of the chosen continuations."""
+    tokens: torch.Tensor    # int64
+    parents: torch.Tensor   # int32, the beam each one continues
+    scores: torch.Tensor    # float32 summed log-probabilities
+    finished: torch.Tensor  # bool
+    lengths: torch.Tensor   # int32
+
+
+@lru_cache(maxsize=256)
+def _beam_workspace(G: int, W: int, V: int, K: int) -> int:
+    n = ctypes.c_int64(0)
+    _lib.call("tesm_b200_beam_select_workspace", G, W, V, K, ctypes.addressof(n))
+    return n.value
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: Optional[int] = None, *,
+                finished: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
+                eos_token_id: Optional[int] = None, pad_token_id: int = 0,
+                length_penalty: float = 0.0) -> BeamStep:
+    """The best ``beams`` continuations of every prompt's beams (tesm_b200_beam_select).
+
+    logits (prompts, W, vocab) float32 or bfloat16 with unit vocabulary stride, scores (prompts, W)
+    float32.  A live beam offers ``scores + log_softmax(logits)`` for every token, a ``finished`` one
+    (bool) only itself with ``pad_token_id``; they are ranked by score / length ** length_penalty with
+    ``lengths`` (int32) counting the new token, ties to the lower beam, then the lower token.  Beams
+    start as ``scores = [0, -inf, ...]``: candidates of score -inf never win, and slots that
+    nothing is left for come back finished with score -inf.  ``beams`` defaults to W; both at most 32."""
+    what = "beam_select"
+    _need(logits.dim() == 3, f"{what}: logits must be (prompts, beams, vocab), got {tuple(logits.shape)}")
+    G, W, V = logits.shape
+    K = W if beams is None else int(beams)
+    dt = dtype_code(logits.dtype)
+    dev = logits.device
+    _need(logits.is_cuda, f"{what}: logits must be on a CUDA device")
+    _need(1 <= W <= MAX_BEAMS and 1 <= K <= MAX_BEAMS, f"{what}: 1 to {MAX_BEAMS} beams, got {W} in and {K} out")
+    _need(V >= 1 and (logits.stride(2) == 1 or V == 1), f"{what}: the vocabulary must be there with unit stride")
+    _need(0 <= pad_token_id < V, f"{what}: pad_token_id {pad_token_id} is outside the vocabulary of {V}")
+    _need(length_penalty == 0.0 or lengths is not None, f"{what}: a length penalty needs lengths")
+    _check(what, "scores", scores, (G, W), torch.float32, dev)
+    _check(what, "finished", finished, (G, W), torch.bool, dev)
+    _check(what, "lengths", lengths, (G, W), torch.int32, dev)
+    _no_grad(what, logits, scores)
+    tokens = torch.empty((G, K), device=dev, dtype=torch.int64)
+    parents = torch.empty((G, K), device=dev, dtype=torch.int32)
+    out_scores = torch.empty((G, K), device=dev, dtype=torch.float32)
+    out_finished = torch.empty((G, K), device=dev, dtype=torch.bool)
+    out_lengths = torch.empty((G, K), device=dev, dtype=torch.int32)
+    ws = torch.empty(_beam_workspace(G, W, V, K), device=dev, dtype=torch.uint8)
+    _call_on(dev, "tesm_b200_beam_select", logits.data_ptr(), dt, logits.stride(0) if G > 1 else 0,
+             logits.stride(1) if W > 1 else 0, G, W, V, K, scores.data_ptr(), _ptr(finished), _ptr(lengths),
+             -1 if eos_token_id is None else int(eos_token_id), int(pad_token_id), float(length_penalty),
+             tokens.data_ptr(), parents.data_ptr(), out_scores.data_ptr(), out_finished.data_ptr(),
+             out_lengths.data_ptr(), ws.data_ptr(), ws.numel())
+    return BeamStep(tokens, parents, out_scores, out_finished, out_lengths)
+
+
+def _row_layout(what: str, t: torch.Tensor, rows: int):
+    """(data pointer, row bytes, row stride in bytes) of a tensor whose rows are dense."""
+    _need(t.dim() >= 1 and t.shape[0] == rows, f"{what}: a state of shape {tuple(t.shape)} has not {rows} rows")
+    n = 1
+    for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+        _need(size == 1 or stride == n, f"{what}: the rows of a state must be dense (shape {tuple(t.shape)}, strides "
+                                        f"{t.stride()})")
+        n *= size
+    es = t.element_size()
+    stride = t.stride(0) if rows > 1 else n
+    _need(stride >= n, f"{what}: the rows of a state overlap")
+    return t.data_ptr(), n * es, stride * es
+
+
+def _rows_disjoint(a, b) -> bool:
+    """Whether two (pointer, row bytes, stride, rows) sets of rows share no byte."""
+    (pa, na, sa, ra), (pb, nb, sb, rb) = sorted((a, b))
+    if not na or not nb or not ra or not rb or pa + (ra - 1) * sa + na <= pb:
+        return True
+    off = (pb - pa) % sa
+    return sa == sb and off >= na and off + nb <= sa  # interleaved columns of one buffer
+
+
+class StateReorder:
+    """Moves the rows of a fixed set of state tensors along with their beams, in place.
+
+    ``states``: tensors of prompts * beams rows (any type and row shape; rows dense, any row
+    stride), e.g. the caches of all layers.  ``plan(parents)`` with parents (prompts, beams) int32
+    makes row g * beams + k of every state the row g * beams + parents[g, k], all in one launch per 128
+    tensors; each column of rows is read into registers before it is stored, so no copy is kept.
+    With ``out`` (tensors of prompts * beams rows) the rows come from ``states`` of prompts * ``beams_in``
+    rows instead: beams_in = 1 and parents of zeros spreads one row per prompt over its beams.
+    A parent out of range leaves its row as it is and sets :func:`device_status` to 1."""
+
+    def __init__(self, states: Sequence[torch.Tensor], beams: int, out: Optional[Sequence[torch.Tensor]] = None,
+                 beams_in: Optional[int] = None):
+        what = "reorder_states"
+        states = list(states)
+        dst = states if out is None else list(out)
+        beams_in = beams if beams_in is None else int(beams_in)
+        _need(len(states) > 0, f"{what}: no states")
+        _need(1 <= beams <= MAX_BEAMS, f"{what}: 1 to {MAX_BEAMS} beams, got {beams}")
+        _need(beams_in >= 1 and (out is not None or beams_in == beams), f"{what}: in place, beams_in equals beams")
+        _need(len(dst) == len(states), f"{what}: {len(states)} states but {len(dst)} outputs")
+        self.device = states[0].device
+        _need(all(t.is_cuda and t.device == self.device for t in states + dst),
+              f"{what}: all states must be on one CUDA device")
+        rows_in = states[0].shape[0] if states[0].dim() else 0
+        _need(rows_in % beams_in == 0, f"{what}: {rows_in} rows are no multiple of {beams_in} beams")
+        self.prompts, self.beams, self.beams_in = rows_in // beams_in, int(beams), beams_in
+        rows_out = self.prompts * self.beams
+        self._table = (_lib.StateRows * len(states))()
+        src_rows, dst_rows = [], []
+        for e, s, d in zip(self._table, states, dst):
+            _need(s.dtype == d.dtype and s.shape[1:] == d.shape[1:], f"{what}: a state and its output differ in type or "
+                                                                     f"row shape")
+            _no_grad(what, s, d)
+            e.src, e.row_bytes, e.src_stride = _row_layout(what, s, rows_in)
+            e.dst, _, e.dst_stride = _row_layout(what, d, rows_out)
+            src_rows.append((s.data_ptr(), e.row_bytes, e.src_stride, rows_in))
+            dst_rows.append((d.data_ptr(), e.row_bytes, e.dst_stride, rows_out))
+        # what is written is written once, and nothing that another entry reads
+        for i, d in enumerate(dst_rows):
+            for other in dst_rows[:i] + (src_rows if out is not None else []):
+                _need(_rows_disjoint(d, other), f"{what}: states share memory")
+        self._keep = (states, dst)
+
+    def __call__(self, parents: torch.Tensor):
+        _check("reorder_states", "parents", parents, (self.prompts, self.beams), torch.int32, self.device)
+        _call_on(self.device, "tesm_b200_reorder_states", ctypes.addressof(self._table), len(self._table), self.prompts,
+                 self.beams_in, self.beams, parents.data_ptr())
+        return self._keep[1]
+
+
+def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor, out: Optional[Sequence[torch.Tensor]] = None):
+    """One :class:`StateReorder` call; a loop keeps the plan.  Returns the reordered tensors."""
+    _need(parents.dim() == 2 and parents.shape[0] > 0, "reorder_states: parents must be (prompts, beams)")
+    states = list(states)
+    _need(len(states) > 0 and states[0].dim() > 0 and states[0].shape[0] % parents.shape[0] == 0,
+          f"reorder_states: the states' rows are no multiple of {parents.shape[0]} prompts")
+    return StateReorder(states, parents.shape[1], out, None if out is None else
+                        states[0].shape[0] // parents.shape[0])(parents)
+
+
+# ------------------------------------------------------------------ selective state space scan
+def _rows3(what: str, name: str, t: Optional[torch.Tensor], shape, dtype, dev):
+    """(batch, token) element strides of a (B, L, n) tensor with unit innermost stride."""
+    if t is None:
+        return 0, 0
+    _need(t.shape == shape and t.dtype == dtype and t.device == dev,
+          f"{what}: {name} must be a {dtype} tensor of shape {tuple(shape)} on {dev}, got {t.dtype} {tuple(t.shape)} on "
+          f"{t.device}")
+    _need(shape[2] <= 1 or t.stride(2) == 1, f"{what}: {name} needs unit stride along its last dimension")
+    return t.stride(0) if shape[0] > 1 else 0, t.stride(1) if shape[1] > 1 else 0
+
+
+def _span(t: torch.Tensor):
+    """First and one-past-last byte address of a tensor's elements."""
+    if t.numel() == 0:
+        return 0, 0
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _check_written(what: str, name: str, t: torch.Tensor, *others):
+    """A tensor that the kernel writes: no element twice, and none of ``others``' memory range."""
+    at = 1  # strides in increasing order each step over all that lies below them
+    for stride, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
+        _need(stride >= at, f"{what}: {name} overlaps itself")
+        at = stride * (n - 1) + at
+    a0, a1 = _span(t)
+    for o in others:
+        if o is not None:
+            b0, b1 = _span(o)
+            _need(a1 <= b0 or b1 <= a0 or a0 == a1 or b0 == b1, f"{what}: {name} shares memory with another argument")
+
+
+def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
+                state: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None, silu: bool = True,
+                out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Short causal depthwise convolution of a prompt, or of one token (L = 1), with SiLU.
+
+    x (B, L, D) float32 or bfloat16 with unit channel stride; weight (D, K) float32, K = 2 .. 8, the last
+    tap on the current token; bias (D,) float32.  ``state`` (B, K - 1, D) of x's type holds the inputs
+    before the first token (zeros if not given) and is replaced by the last K - 1 inputs.
+    ``lengths`` (B,) int32: tokens of each sequence (right-padded); outputs behind them are zeros."""
+    what = "causal_conv"
+    _need(x.dim() == 3 and x.is_cuda, f"{what}: x must be a (batch, tokens, channels) CUDA tensor")
+    B, L, D = x.shape
+    dev, dt = x.device, dtype_code(x.dtype)
+    xb, xl = _rows3(what, "x", x, (B, L, D), x.dtype, dev)
+    _need(weight.dim() == 2 and 2 <= weight.shape[1] <= 8, f"{what}: weight must be (channels, 2 to 8 taps), got "
+                                                           f"{tuple(weight.shape)}")
+    K = weight.shape[1]
+    _check(what, "weight", weight, (D, K), torch.float32, dev)
+    _check(what, "bias", bias, (D,), torch.float32, dev)
+    _check(what, "state", state, (B, K - 1, D), x.dtype, dev)
+    _check(what, "lengths", lengths, (B,), torch.int32, dev)
+    _no_grad(what, x, weight, bias)
+    if out is None:
+        out = torch.empty((B, L, D), device=dev, dtype=x.dtype)
+        ob, ol = L * D, D
+    else:
+        ob, ol = _rows3(what, "out", out, (B, L, D), x.dtype, dev)
+        _check_written(what, "out", out, x, weight, bias, state, lengths)
+    if state is not None:
+        _check_written(what, "state", state, x, weight, bias, lengths)
+    _call_on(dev, "tesm_b200_causal_conv", x.data_ptr(), dt, xb, xl, B, L, D, K, weight.data_ptr(), _ptr(bias),
+             _ptr(state), _ptr(lengths), int(silu), out.data_ptr(), ob, ol)
+    return out
+
+
+def ssm_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, Bm: torch.Tensor, Cm: torch.Tensor, *,
+             D: Optional[torch.Tensor] = None, z: Optional[torch.Tensor] = None,
+             dt_bias: Optional[torch.Tensor] = None, softplus: bool = True, state: Optional[torch.Tensor] = None,
+             lengths: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Selective state space scan of a prompt, or of one token (L = 1):
+
+        dt = softplus(dt + dt_bias);  h = exp(dt A) h + (dt x) Bm;  y = Cm . h + D x;  out = y silu(z)
+
+    x, dt, z (B, L, channels) and Bm, Cm (B, L, N) of one type (float32 or bfloat16) with unit
+    innermost stride, so slices of a projection are taken as they are; A (channels, N), D and dt_bias
+    (channels,) float32; N = 1 .. 128.  ``state`` (B, channels, N) float32 holds h before the first token
+    (zeros if not given) and is replaced by h after the last.  ``lengths`` (B,) int32: tokens of each
+    sequence (right-padded); outputs behind them are zeros and do not touch the state."""
+    what = "ssm_scan"
+    _need(x.dim() == 3 and x.is_cuda, f"{what}: x must be a (batch, tokens, channels) CUDA tensor")
+    B, L, C = x.shape
+    _need(A.dim() == 2 and 1 <= A.shape[1] <= 128, f"{what}: A must be (channels, 1 to 128 states), got "
+                                                   f"{tuple(A.shape)}")
+    N = A.shape[1]
+    dev, code = x.device, dtype_code(x.dtype)
+    ld = _rows3(what, "x", x, (B, L, C), x.dtype, dev) + _rows3(what, "dt", dt, (B, L, C), x.dtype, dev) + \
+        _rows3(what, "Bm", Bm, (B, L, N), x.dtype, dev) + _rows3(what, "Cm", Cm, (B, L, N), x.dtype, dev) + \
+        _rows3(what, "z", z, (B, L, C), x.dtype, dev)
+    _check(what, "A", A, (C, N), torch.float32, dev)
+    _check(what, "D", D, (C,), torch.float32, dev)
+    _check(what, "dt_bias", dt_bias, (C,), torch.float32, dev)
+    _check(what, "state", state, (B, C, N), torch.float32, dev)
+    _check(what, "lengths", lengths, (B,), torch.int32, dev)
+    _no_grad(what, x, dt, A, Bm, Cm, D, z, dt_bias, state)
+    if out is None:
+        out = torch.empty((B, L, C), device=dev, dtype=x.dtype)
+        ld += (L * C, C)
+    else:
+        ld += _rows3(what, "out", out, (B, L, C), x.dtype, dev)
+        _check_written(what, "out", out, x, dt, A, Bm, Cm, D, z, dt_bias, state, lengths)
+    if state is not None:
+        _check_written(what, "state", state, x, dt, A, Bm, Cm, D, z, dt_bias, lengths)
+    strides = (ctypes.c_int64 * 12)(*ld)
+    _call_on(dev, "tesm_b200_ssm_scan", x.data_ptr(), dt.data_ptr(), Bm.data_ptr(), Cm.data_ptr(), _ptr(z),
+             out.data_ptr(), ctypes.addressof(strides), code, B, L, C, N, A.data_ptr(), _ptr(D), _ptr(dt_bias),
+             int(softplus), _ptr(state), _ptr(lengths))
+    return out

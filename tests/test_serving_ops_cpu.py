@@ -1,0 +1,132 @@
+"""Refusals of the beam and scan entry points, and the host-side checks, without a GPU."""
+import ctypes
+
+import pytest
+import torch
+
+from tesm_b200 import _lib, ops
+
+P = ctypes.c_void_p(4096)  # never dereferenced: the checks come first
+
+
+def status(name, *args):
+    return getattr(_lib.load(), name)(*args)
+
+
+def beam(dtype=0, G=1, W=4, V=100, K=4, logits=P, scores=P, lengths=None, alpha=0.0, pad=0, ws=P, ws_bytes=1 << 30):
+    return status("tesm_b200_beam_select", logits, dtype, 400, 100, G, W, V, K, scores, None, lengths, -1, pad, alpha, P, P,
+                  P, P, P, ws, ws_bytes, None)
+
+
+@pytest.mark.parametrize("kw,want", [(dict(dtype=2), 2), (dict(W=0), 1), (dict(W=33), 1), (dict(K=0), 1), (dict(K=33), 1),
+                                     (dict(V=0), 1), (dict(V=1 << 31), 1), (dict(G=-1), 1), (dict(G=1 << 23), 1),
+                                     (dict(logits=None), 1), (dict(scores=None), 1), (dict(alpha=1.0), 1),
+                                     (dict(alpha=float("nan"), lengths=P), 1), (dict(pad=-1), 1), (dict(ws=None), 1),
+                                     (dict(ws_bytes=15), 1), (dict(ws=ctypes.c_void_p(4104)), 1), (dict(G=0), 0)])
+def test_beam_select_refuses(kw, want):
+    assert beam(**kw) == want
+    if want:
+        assert "beam_select" in _lib.last_error()
+
+
+def test_beam_workspace():
+    n = ctypes.c_int64(-1)
+    assert status("tesm_b200_beam_select_workspace", 2, 4, 32000, 4, ctypes.addressof(n)) == 0 and n.value > 0
+    assert status("tesm_b200_beam_select_workspace", 0, 4, 32000, 4, ctypes.addressof(n)) == 0 and n.value == 0
+    assert status("tesm_b200_beam_select_workspace", 2, 33, 32000, 4, ctypes.addressof(n)) == 1
+    assert status("tesm_b200_beam_select_workspace", 2, 4, 32000, 4, None) == 1
+
+
+def rows(*entries):
+    t = (_lib.StateRows * len(entries))()
+    for e, (src, dst, n, s, d) in zip(t, entries):
+        e.src, e.dst, e.row_bytes, e.src_stride, e.dst_stride = src, dst, n, s, d
+    return t
+
+
+@pytest.mark.parametrize("entry,G,Win,Wout,parents,want", [
+    ((4096, 4096, 64, 64, 64), 2, 4, 33, P, 1), ((4096, 4096, 64, 64, 64), 2, 4, 0, P, 1),
+    ((4096, 4096, 64, 64, 64), 2, 0, 4, P, 1), ((4096, 4096, 64, 64, 64), -1, 4, 4, P, 1),
+    ((4096, 4096, 64, 64, 64), 2, 4, 4, None, 1), ((None, 4096, 64, 64, 64), 2, 4, 4, P, 1),
+    ((4096, None, 64, 64, 64), 2, 4, 4, P, 1), ((4096, 4096, 64, 32, 64), 2, 4, 4, P, 1),
+    ((4096, 4096, 64, 64, 32), 2, 4, 4, P, 1), ((4096, 4096, -1, 64, 64), 2, 4, 4, P, 1),
+    ((4096, 4096, 64, 64, 64), 2, 1, 4, P, 1), ((4096, 4096, 64, 64, 128), 2, 4, 4, P, 1),
+    ((4096, 4096, 1 << 36, 1 << 36, 1 << 36), 2, 4, 4, P, 5), ((4096, 4096, 64, 64, 64), 0, 4, 4, P, 0),
+    ((4096, 4096, 0, 0, 0), 2, 4, 4, P, 0)])
+def test_reorder_refuses(entry, G, Win, Wout, parents, want):
+    t = rows(entry)
+    assert status("tesm_b200_reorder_states", ctypes.addressof(t), 1, G, Win, Wout, parents, None) == want
+
+
+def test_reorder_refuses_no_table():
+    assert status("tesm_b200_reorder_states", None, 1, 2, 4, 4, P, None) == 1
+    assert status("tesm_b200_reorder_states", None, 0, 2, 4, 4, P, None) == 0
+
+
+def conv(dtype=0, B=1, L=4, D=8, K=4, x=P, w=P, out=P):
+    return status("tesm_b200_causal_conv", x, dtype, 32, 8, B, L, D, K, w, None, None, None, 1, out, 32, 8, None)
+
+
+@pytest.mark.parametrize("kw,want", [(dict(dtype=3), 2), (dict(B=-1), 1), (dict(L=-1), 1), (dict(D=1 << 31), 1),
+                                     (dict(K=1), 5), (dict(K=9), 5), (dict(x=None), 1), (dict(w=None), 1),
+                                     (dict(out=None), 1), (dict(B=1 << 29, L=64, D=1024), 1), (dict(L=0), 0), (dict(B=0), 0)])
+def test_conv_refuses(kw, want):
+    assert conv(**kw) == want
+
+
+def scan(dtype=0, B=1, L=4, D=8, N=16, x=P, A=P, out=P, strides=True):
+    s = (ctypes.c_int64 * 12)(*[64] * 12)
+    return status("tesm_b200_ssm_scan", x, P, P, P, None, out, ctypes.addressof(s) if strides else None, dtype, B, L, D, N,
+                  A, None, None, 1, None, None, None)
+
+
+@pytest.mark.parametrize("kw,want", [(dict(dtype=3), 2), (dict(B=-1), 1), (dict(L=1 << 30), 1), (dict(N=0), 5),
+                                     (dict(N=129), 5), (dict(x=None), 1), (dict(A=None), 1), (dict(out=None), 1),
+                                     (dict(strides=False), 1), (dict(B=1 << 29, D=64), 1), (dict(L=0), 0), (dict(D=0), 0)])
+def test_scan_refuses(kw, want):
+    assert scan(**kw) == want
+
+
+def test_rows_disjoint():
+    """Sets of rows (pointer, bytes, stride, rows): apart, interleaved in one buffer, overlapping."""
+    d = ops._rows_disjoint
+    assert d((0, 8, 8, 4), (32, 8, 8, 4)) and not d((0, 8, 8, 4), (24, 8, 8, 4))
+    assert d((0, 8, 16, 4), (8, 8, 16, 4)) and d((8, 8, 16, 4), (0, 8, 16, 4))
+    assert not d((0, 8, 16, 4), (4, 8, 16, 4)) and not d((0, 8, 16, 4), (12, 8, 16, 4))
+    assert not d((0, 8, 16, 4), (8, 8, 24, 4)) and not d((0, 8, 8, 1), (0, 8, 8, 1))
+    assert d((0, 0, 8, 4), (0, 8, 8, 4)) and d((0, 8, 8, 0), (0, 8, 8, 4))
+    # by brute force
+    g = torch.Generator().manual_seed(0)
+    for _ in range(300):
+        a, b = ([int(v) for v in torch.randint(0, 20, (4,), generator=g)] for _ in range(2))
+        for t in (a, b):
+            t[2] = max(t[1], 1) + t[2] % 5
+            t[3] = t[3] % 4
+        if int(torch.randint(0, 2, (1,), generator=g)):
+            b[2] = max(a[2], b[1])
+        cover = [set(p + r * s + i for r in range(k) for i in range(n)) for p, n, s, k in (a, b)]
+        if ops._rows_disjoint(tuple(a), tuple(b)):
+            assert not (cover[0] & cover[1]), (a, b)
+
+
+def test_written_tensors_are_checked():
+    x = torch.zeros(2, 5, 8)
+    ops._check_written("op", "out", torch.zeros(2, 5, 8), x)
+    ops._check_written("op", "out", torch.zeros(5, 2, 8).transpose(0, 1), x, None)
+    ops._check_written("op", "out", torch.zeros(0, 5, 8), x)
+    for out in (x, x[:, 1:], torch.zeros(1, 5, 8).expand(2, 5, 8), torch.zeros(20).as_strided((2, 5, 8), (1, 1, 1)),
+                torch.zeros(100).as_strided((2, 5, 8), (36, 8, 1))):
+        with pytest.raises(ValueError):
+            ops._check_written("op", "out", out, x)
+
+
+def test_cpu_tensors_are_refused():
+    z = torch.zeros
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.beam_select(z(1, 2, 8), z(1, 2))
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.StateReorder([z(4, 3)], 2)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.causal_conv(z(1, 2, 8), z(8, 4))
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.ssm_scan(z(1, 2, 8), z(1, 2, 8), z(8, 4), z(1, 2, 4), z(1, 2, 4))
