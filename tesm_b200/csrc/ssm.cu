@@ -85,6 +85,25 @@ __device__ __forceinline__ int seq_len(const int *lengths, int64_t b, int L) {
   return lengths ? min(max(lengths[b], 0), L) : L;
 }
 
+// ------------------------------------------------------------ host-side checks of what is written
+struct Span {
+  uintptr_t lo, hi;
+  bool meets(const Span &o) const { return lo < o.hi && o.lo < hi; }
+};
+// bytes of a (B, L, n) tensor of `es`-byte elements with element strides ldb, ldl
+static Span span3(const void *p, int64_t B, int64_t L, int64_t n, int64_t ldb, int64_t ldl, int64_t es) {
+  if (!p) return Span{0, 0};
+  const uintptr_t lo = (uintptr_t)p;
+  return Span{lo, lo + (uintptr_t)(((B - 1) * ldb + (L - 1) * ldl + n) * es)};
+}
+static Span span1(const void *p, int64_t bytes) { return p ? Span{(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes} : Span{0, 0}; }
+// whether a (B, L, n) tensor holds an element twice
+static bool self_overlap(int64_t B, int64_t L, int64_t n, int64_t ldb, int64_t ldl) {
+  if (B > 1 && L > 1)
+    return ldb < ldl ? ldb < n || ldl < (B - 1) * ldb + n : ldl < n || ldb < (L - 1) * ldl + n;
+  return (B > 1 && ldb < n) || (L > 1 && ldl < n);
+}
+
 // ------------------------------------------------------------ causal convolution
 // y_t = act(bias + sum_j w_j x_{t-K+1+j}).  A thread owns N channels (16 bytes of them) and walks
 // a tile of tokens with the last K - 1 inputs in registers, so x is read once (and K - 1 rows
@@ -481,6 +500,14 @@ extern "C" int tesm_b200_causal_conv(const void *x, int dtype, int64_t ldxb, int
   if (B == 0 || L == 0 || D == 0) return TESM_OK;
   TESM_REQUIRE(x && weight && out, "causal_conv: null pointer");
   TESM_REQUIRE(B * ceil_div(D, kConvThreads) * ceil_div(L, 8) < (1ll << 31), "causal_conv: too many blocks");
+  const int64_t es = dtype == TESM_BF16 ? 2 : 4;
+  TESM_REQUIRE(ldxb >= 0 && ldxl >= 0 && ldob >= 0 && ldol >= 0, "causal_conv: negative stride");
+  TESM_REQUIRE(!self_overlap(B, L, D, ldob, ldol), "causal_conv: out overlaps itself");
+  const Span so = span3(out, B, L, D, ldob, ldol, es), ss = span1(state, B * (K - 1) * D * es);
+  for (const Span &r : {span3(x, B, L, D, ldxb, ldxl, es), span1(weight, D * K * 4), span1(bias, D * 4),
+                        span1(lengths, B * 4)})
+    TESM_REQUIRE(!so.meets(r) && !ss.meets(r), "causal_conv: out or state shares memory with an input");
+  TESM_REQUIRE(!so.meets(ss), "causal_conv: out shares memory with state");
   cudaStream_t st = (cudaStream_t)stream;
   return dtype == TESM_BF16 ? causal_conv_t<__nv_bfloat16>(x, ldxb, ldxl, B, L, D, K, weight, bias, state, lengths, silu,
                                                            out, ldob, ldol, st)
@@ -521,6 +548,16 @@ extern "C" int tesm_b200_ssm_scan(const void *x, const void *dt, const void *bm,
   if (B == 0 || L == 0 || D == 0) return TESM_OK;
   TESM_REQUIRE(x && dt && bm && cm && out && A && strides, "ssm_scan: null pointer");
   TESM_REQUIRE(B * ceil_div(D, 4) < (1ll << 31), "ssm_scan: too many blocks");
+  const int64_t es = dtype == TESM_BF16 ? 2 : 4, *ld = strides;
+  for (int i = 0; i < 12; ++i) TESM_REQUIRE(ld[i] >= 0, "ssm_scan: negative stride");
+  TESM_REQUIRE(!self_overlap(B, L, D, ld[10], ld[11]), "ssm_scan: out overlaps itself");
+  const Span so = span3(out, B, L, D, ld[10], ld[11], es), ss = span1(state, B * D * N * 4);
+  for (const Span &r : {span3(x, B, L, D, ld[0], ld[1], es), span3(dt, B, L, D, ld[2], ld[3], es),
+                        span3(bm, B, L, N, ld[4], ld[5], es), span3(cm, B, L, N, ld[6], ld[7], es),
+                        span3(z, B, L, D, ld[8], ld[9], es), span1(A, D * N * 4), span1(skip, D * 4),
+                        span1(dt_bias, D * 4), span1(lengths, B * 4)})
+    TESM_REQUIRE(!so.meets(r) && !ss.meets(r), "ssm_scan: out or state shares memory with an input");
+  TESM_REQUIRE(!so.meets(ss), "ssm_scan: out shares memory with state");
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == TESM_BF16) {
     ScanArgs<__nv_bfloat16> a = {};

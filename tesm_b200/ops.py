@@ -515,26 +515,25 @@ def _need(ok, what: str):
 
 
 def _no_grad(what: str, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"tesm_b200 {what} has no autograd path (use torch.no_grad())")
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"tesm_b200 {what} has no autograd path (use torch.no_grad())")
 
 
-def _call_on(dev: torch.device, name: str, *args):
-    """Launch on ``dev``'s current stream, whichever device is current."""
-    if dev.index == torch.cuda.current_device():
-        _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+def _call_on(index: int, name: str, *args):
+    """Launch on the current stream of device ``index``, whichever device is current."""
+    if index == torch.cuda.current_device():
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(dev):
-            _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(index):
+            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
-def _check(what: str, name: str, t: Optional[torch.Tensor], shape, dtype: torch.dtype, dev: torch.device):
-    """A dense tensor of this shape, type and device (or None)."""
-    if t is None:
-        return
-    _need(t.shape == shape and t.dtype == dtype and t.device == dev and t.is_contiguous(),
-          f"{what}: {name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {dev}, got "
-          f"{t.dtype} {tuple(t.shape)} on {t.device}")
+def _check(what: str, name: str, t: Optional[torch.Tensor], shape, dtype: torch.dtype, index: int):
+    """A dense tensor of this shape and type on device ``index`` (or None)."""
+    if t is not None and (t.shape != shape or t.dtype != dtype or t.get_device() != index or not t.is_contiguous()):
+        raise ValueError(f"tesm_b200 {what}: {name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on "
+                         f"cuda:{index}, got {t.dtype} {tuple(t.shape)} {t.stride()} on {t.device}")
 
 
 @dataclass
@@ -567,31 +566,37 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: Optional[int]
     start as ``scores = [0, -inf, ...]``: candidates of score -inf never win, and slots that
     nothing is left for come back finished with score -inf.  ``beams`` defaults to W; both at most 32."""
     what = "beam_select"
-    _need(logits.dim() == 3, f"{what}: logits must be (prompts, beams, vocab), got {tuple(logits.shape)}")
+    if logits.dim() != 3 or not logits.is_cuda:
+        raise ValueError(f"tesm_b200 {what}: logits must be a (prompts, beams, vocab) CUDA tensor, got "
+                         f"{tuple(logits.shape)} on {logits.device}")
     G, W, V = logits.shape
     K = W if beams is None else int(beams)
-    dt = dtype_code(logits.dtype)
-    dev = logits.device
-    _need(logits.is_cuda, f"{what}: logits must be on a CUDA device")
-    _need(1 <= W <= MAX_BEAMS and 1 <= K <= MAX_BEAMS, f"{what}: 1 to {MAX_BEAMS} beams, got {W} in and {K} out")
-    _need(V >= 1 and (logits.stride(2) == 1 or V == 1), f"{what}: the vocabulary must be there with unit stride")
-    _need(0 <= pad_token_id < V, f"{what}: pad_token_id {pad_token_id} is outside the vocabulary of {V}")
-    _need(length_penalty == 0.0 or lengths is not None, f"{what}: a length penalty needs lengths")
+    code, dev = dtype_code(logits.dtype), logits.get_device()
+    if not (1 <= W <= MAX_BEAMS and 1 <= K <= MAX_BEAMS):
+        raise ValueError(f"tesm_b200 {what}: 1 to {MAX_BEAMS} beams, got {W} in and {K} out")
+    ldg, ldw, ldv = logits.stride()
+    if V < 1 or (ldv != 1 and V > 1):
+        raise ValueError(f"tesm_b200 {what}: the logits need unit stride over a vocabulary, got {logits.stride()}")
+    if not 0 <= pad_token_id < V:
+        raise ValueError(f"tesm_b200 {what}: pad_token_id {pad_token_id} is outside the vocabulary of {V}")
+    if length_penalty != 0.0 and lengths is None:
+        raise ValueError(f"tesm_b200 {what}: a length penalty needs lengths")
     _check(what, "scores", scores, (G, W), torch.float32, dev)
     _check(what, "finished", finished, (G, W), torch.bool, dev)
     _check(what, "lengths", lengths, (G, W), torch.int32, dev)
     _no_grad(what, logits, scores)
-    tokens = torch.empty((G, K), device=dev, dtype=torch.int64)
-    parents = torch.empty((G, K), device=dev, dtype=torch.int32)
-    out_scores = torch.empty((G, K), device=dev, dtype=torch.float32)
-    out_finished = torch.empty((G, K), device=dev, dtype=torch.bool)
-    out_lengths = torch.empty((G, K), device=dev, dtype=torch.int32)
-    ws = torch.empty(_beam_workspace(G, W, V, K), device=dev, dtype=torch.uint8)
-    _call_on(dev, "tesm_b200_beam_select", logits.data_ptr(), dt, logits.stride(0) if G > 1 else 0,
-             logits.stride(1) if W > 1 else 0, G, W, V, K, scores.data_ptr(), _ptr(finished), _ptr(lengths),
-             -1 if eos_token_id is None else int(eos_token_id), int(pad_token_id), float(length_penalty),
-             tokens.data_ptr(), parents.data_ptr(), out_scores.data_ptr(), out_finished.data_ptr(),
-             out_lengths.data_ptr(), ws.data_ptr(), ws.numel())
+    out = (G, K)
+    tokens = scores.new_empty(out, dtype=torch.int64)
+    parents = scores.new_empty(out, dtype=torch.int32)
+    out_scores = scores.new_empty(out)
+    out_finished = scores.new_empty(out, dtype=torch.bool)
+    out_lengths = scores.new_empty(out, dtype=torch.int32)
+    ws_bytes = _beam_workspace(G, W, V, K)
+    ws = scores.new_empty(ws_bytes, dtype=torch.uint8)
+    _call_on(dev, "tesm_b200_beam_select", logits.data_ptr(), code, ldg if G > 1 else 0, ldw if W > 1 else 0, G, W, V,
+             K, scores.data_ptr(), _ptr(finished), _ptr(lengths), -1 if eos_token_id is None else eos_token_id,
+             pad_token_id, length_penalty, tokens.data_ptr(), parents.data_ptr(), out_scores.data_ptr(),
+             out_finished.data_ptr(), out_lengths.data_ptr(), ws.data_ptr(), ws_bytes)
     return BeamStep(tokens, parents, out_scores, out_finished, out_lengths)
 
 
@@ -639,8 +644,8 @@ class StateReorder:
         _need(1 <= beams <= MAX_BEAMS, f"{what}: 1 to {MAX_BEAMS} beams, got {beams}")
         _need(beams_in >= 1 and (out is not None or beams_in == beams), f"{what}: in place, beams_in equals beams")
         _need(len(dst) == len(states), f"{what}: {len(states)} states but {len(dst)} outputs")
-        self.device = states[0].device
-        _need(all(t.is_cuda and t.device == self.device for t in states + dst),
+        self.device = states[0].get_device()
+        _need(all(t.is_cuda and t.get_device() == self.device for t in states + dst),
               f"{what}: all states must be on one CUDA device")
         rows_in = states[0].shape[0] if states[0].dim() else 0
         _need(rows_in % beams_in == 0, f"{what}: {rows_in} rows are no multiple of {beams_in} beams")
@@ -656,16 +661,21 @@ class StateReorder:
             e.dst, _, e.dst_stride = _row_layout(what, d, rows_out)
             src_rows.append((s.data_ptr(), e.row_bytes, e.src_stride, rows_in))
             dst_rows.append((d.data_ptr(), e.row_bytes, e.dst_stride, rows_out))
-        # what is written is written once, and nothing that another entry reads
-        for i, d in enumerate(dst_rows):
-            for other in dst_rows[:i] + (src_rows if out is not None else []):
-                _need(_rows_disjoint(d, other), f"{what}: states share memory")
+        # what is written is written once, and nothing that another entry reads; sorted by address, a
+        # set of rows can only meet those that begin before its end
+        every = sorted([(r, True) for r in dst_rows] + ([(r, False) for r in src_rows] if out is not None else []))
+        for i, (r, written) in enumerate(every):
+            end = r[0] + (r[3] - 1) * r[2] + r[1]
+            for other, also in every[i + 1:]:
+                if other[0] >= end:
+                    break
+                _need(not (written or also) or _rows_disjoint(r, other), f"{what}: states share memory")
         self._keep = (states, dst)
+        self._args = (ctypes.addressof(self._table), len(states), self.prompts, self.beams_in, self.beams)
 
     def __call__(self, parents: torch.Tensor):
         _check("reorder_states", "parents", parents, (self.prompts, self.beams), torch.int32, self.device)
-        _call_on(self.device, "tesm_b200_reorder_states", ctypes.addressof(self._table), len(self._table), self.prompts,
-                 self.beams_in, self.beams, parents.data_ptr())
+        _call_on(self.device, "tesm_b200_reorder_states", *self._args, parents.data_ptr())
         return self._keep[1]
 
 
@@ -680,36 +690,15 @@ def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor, out: O
 
 
 # ------------------------------------------------------------------ selective state space scan
-def _rows3(what: str, name: str, t: Optional[torch.Tensor], shape, dtype, dev):
+def _rows3(what: str, name: str, t: torch.Tensor, shape, dtype, index: int):
     """(batch, token) element strides of a (B, L, n) tensor with unit innermost stride."""
-    if t is None:
-        return 0, 0
-    _need(t.shape == shape and t.dtype == dtype and t.device == dev,
-          f"{what}: {name} must be a {dtype} tensor of shape {tuple(shape)} on {dev}, got {t.dtype} {tuple(t.shape)} on "
-          f"{t.device}")
-    _need(shape[2] <= 1 or t.stride(2) == 1, f"{what}: {name} needs unit stride along its last dimension")
-    return t.stride(0) if shape[0] > 1 else 0, t.stride(1) if shape[1] > 1 else 0
-
-
-def _span(t: torch.Tensor):
-    """First and one-past-last byte address of a tensor's elements."""
-    if t.numel() == 0:
-        return 0, 0
-    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
-
-
-def _check_written(what: str, name: str, t: torch.Tensor, *others):
-    """A tensor that the kernel writes: no element twice, and none of ``others``' memory range."""
-    at = 1  # strides in increasing order each step over all that lies below them
-    for stride, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
-        _need(stride >= at, f"{what}: {name} overlaps itself")
-        at = stride * (n - 1) + at
-    a0, a1 = _span(t)
-    for o in others:
-        if o is not None:
-            b0, b1 = _span(o)
-            _need(a1 <= b0 or b1 <= a0 or a0 == a1 or b0 == b1, f"{what}: {name} shares memory with another argument")
+    if t.shape != shape or t.dtype != dtype or t.get_device() != index:
+        raise ValueError(f"tesm_b200 {what}: {name} must be a {dtype} tensor of shape {tuple(shape)} on cuda:{index}, got "
+                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
+    b, l, n = t.stride()
+    if n != 1 and shape[2] > 1:
+        raise ValueError(f"tesm_b200 {what}: {name} needs unit stride along its last dimension, got {t.stride()}")
+    return b if shape[0] > 1 else 0, l if shape[1] > 1 else 0
 
 
 def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
@@ -722,28 +711,25 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     before the first token (zeros if not given) and is replaced by the last K - 1 inputs.
     ``lengths`` (B,) int32: tokens of each sequence (right-padded); outputs behind them are zeros."""
     what = "causal_conv"
-    _need(x.dim() == 3 and x.is_cuda, f"{what}: x must be a (batch, tokens, channels) CUDA tensor")
-    B, L, D = x.shape
-    dev, dt = x.device, dtype_code(x.dtype)
-    xb, xl = _rows3(what, "x", x, (B, L, D), x.dtype, dev)
-    _need(weight.dim() == 2 and 2 <= weight.shape[1] <= 8, f"{what}: weight must be (channels, 2 to 8 taps), got "
-                                                           f"{tuple(weight.shape)}")
+    if x.dim() != 3 or not x.is_cuda:
+        raise ValueError(f"tesm_b200 {what}: x must be a (batch, tokens, channels) CUDA tensor")
+    shape, xdt, dev = x.shape, x.dtype, x.get_device()
+    B, L, D = shape
+    code = dtype_code(xdt)
+    xb, xl = _rows3(what, "x", x, shape, xdt, dev)
+    if weight.dim() != 2 or not 2 <= weight.shape[1] <= 8:
+        raise ValueError(f"tesm_b200 {what}: weight must be (channels, 2 to 8 taps), got {tuple(weight.shape)}")
     K = weight.shape[1]
     _check(what, "weight", weight, (D, K), torch.float32, dev)
     _check(what, "bias", bias, (D,), torch.float32, dev)
-    _check(what, "state", state, (B, K - 1, D), x.dtype, dev)
+    _check(what, "state", state, (B, K - 1, D), xdt, dev)
     _check(what, "lengths", lengths, (B,), torch.int32, dev)
     _no_grad(what, x, weight, bias)
     if out is None:
-        out = torch.empty((B, L, D), device=dev, dtype=x.dtype)
-        ob, ol = L * D, D
-    else:
-        ob, ol = _rows3(what, "out", out, (B, L, D), x.dtype, dev)
-        _check_written(what, "out", out, x, weight, bias, state, lengths)
-    if state is not None:
-        _check_written(what, "state", state, x, weight, bias, lengths)
-    _call_on(dev, "tesm_b200_causal_conv", x.data_ptr(), dt, xb, xl, B, L, D, K, weight.data_ptr(), _ptr(bias),
-             _ptr(state), _ptr(lengths), int(silu), out.data_ptr(), ob, ol)
+        out = x.new_empty(shape)
+    ob, ol = _rows3(what, "out", out, shape, xdt, dev)
+    _call_on(dev, "tesm_b200_causal_conv", x.data_ptr(), code, xb, xl, B, L, D, K, weight.data_ptr(), _ptr(bias),
+             _ptr(state), _ptr(lengths), silu, out.data_ptr(), ob, ol)
     return out
 
 
@@ -761,31 +747,28 @@ def ssm_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, Bm: torch.Tenso
     (zeros if not given) and is replaced by h after the last.  ``lengths`` (B,) int32: tokens of each
     sequence (right-padded); outputs behind them are zeros and do not touch the state."""
     what = "ssm_scan"
-    _need(x.dim() == 3 and x.is_cuda, f"{what}: x must be a (batch, tokens, channels) CUDA tensor")
-    B, L, C = x.shape
-    _need(A.dim() == 2 and 1 <= A.shape[1] <= 128, f"{what}: A must be (channels, 1 to 128 states), got "
-                                                   f"{tuple(A.shape)}")
+    if x.dim() != 3 or not x.is_cuda:
+        raise ValueError(f"tesm_b200 {what}: x must be a (batch, tokens, channels) CUDA tensor")
+    shape, xdt, dev = x.shape, x.dtype, x.get_device()
+    B, L, C = shape
+    code = dtype_code(xdt)
+    if A.dim() != 2 or not 1 <= A.shape[1] <= 128:
+        raise ValueError(f"tesm_b200 {what}: A must be (channels, 1 to 128 states), got {tuple(A.shape)}")
     N = A.shape[1]
-    dev, code = x.device, dtype_code(x.dtype)
-    ld = _rows3(what, "x", x, (B, L, C), x.dtype, dev) + _rows3(what, "dt", dt, (B, L, C), x.dtype, dev) + \
-        _rows3(what, "Bm", Bm, (B, L, N), x.dtype, dev) + _rows3(what, "Cm", Cm, (B, L, N), x.dtype, dev) + \
-        _rows3(what, "z", z, (B, L, C), x.dtype, dev)
+    if out is None:
+        out = x.new_empty(shape)
+    bc = (B, L, N)
+    strides = (ctypes.c_int64 * 12)(*_rows3(what, "x", x, shape, xdt, dev), *_rows3(what, "dt", dt, shape, xdt, dev),
+                                    *_rows3(what, "Bm", Bm, bc, xdt, dev), *_rows3(what, "Cm", Cm, bc, xdt, dev),
+                                    *((0, 0) if z is None else _rows3(what, "z", z, shape, xdt, dev)),
+                                    *_rows3(what, "out", out, shape, xdt, dev))
     _check(what, "A", A, (C, N), torch.float32, dev)
     _check(what, "D", D, (C,), torch.float32, dev)
     _check(what, "dt_bias", dt_bias, (C,), torch.float32, dev)
     _check(what, "state", state, (B, C, N), torch.float32, dev)
     _check(what, "lengths", lengths, (B,), torch.int32, dev)
     _no_grad(what, x, dt, A, Bm, Cm, D, z, dt_bias, state)
-    if out is None:
-        out = torch.empty((B, L, C), device=dev, dtype=x.dtype)
-        ld += (L * C, C)
-    else:
-        ld += _rows3(what, "out", out, (B, L, C), x.dtype, dev)
-        _check_written(what, "out", out, x, dt, A, Bm, Cm, D, z, dt_bias, state, lengths)
-    if state is not None:
-        _check_written(what, "state", state, x, dt, A, Bm, Cm, D, z, dt_bias, lengths)
-    strides = (ctypes.c_int64 * 12)(*ld)
     _call_on(dev, "tesm_b200_ssm_scan", x.data_ptr(), dt.data_ptr(), Bm.data_ptr(), Cm.data_ptr(), _ptr(z),
-             out.data_ptr(), ctypes.addressof(strides), code, B, L, C, N, A.data_ptr(), _ptr(D), _ptr(dt_bias),
-             int(softplus), _ptr(state), _ptr(lengths))
+             out.data_ptr(), strides, code, B, L, C, N, A.data_ptr(), _ptr(D), _ptr(dt_bias), softplus, _ptr(state),
+             _ptr(lengths))
     return out

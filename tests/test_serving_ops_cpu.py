@@ -109,15 +109,40 @@ def test_rows_disjoint():
             assert not (cover[0] & cover[1]), (a, b)
 
 
-def test_written_tensors_are_checked():
-    x = torch.zeros(2, 5, 8)
-    ops._check_written("op", "out", torch.zeros(2, 5, 8), x)
-    ops._check_written("op", "out", torch.zeros(5, 2, 8).transpose(0, 1), x, None)
-    ops._check_written("op", "out", torch.zeros(0, 5, 8), x)
-    for out in (x, x[:, 1:], torch.zeros(1, 5, 8).expand(2, 5, 8), torch.zeros(20).as_strided((2, 5, 8), (1, 1, 1)),
-                torch.zeros(100).as_strided((2, 5, 8), (36, 8, 1))):
-        with pytest.raises(ValueError):
-            ops._check_written("op", "out", out, x)
+def vp(n):
+    return None if n is None else ctypes.c_void_p(n)
+
+
+@pytest.mark.parametrize("x,w,state,lengths,out,ldo", [
+    (4096, 1 << 16, None, None, 4096, (32, 8)), (4096, 1 << 16, None, None, 4096 + 4, (32, 8)),
+    (4096, 1 << 16, None, None, 4096 + 252, (32, 8)), (4096, 1 << 16, 8192, None, 8192 + 188, (32, 8)),
+    (4096, 1 << 16, 4096 + 255, None, 1 << 17, (32, 8)), (4096, 8192, None, None, 8192 + 124, (32, 8)),
+    (4096, 8192, None, 1 << 17, (1 << 17) + 4, (32, 8)), (4096, 8192, None, None, 1 << 17, (32, 7)),
+    (4096, 8192, None, None, 1 << 17, (8, 8)), (4096, 8192, None, None, 1 << 17, (0, 8)),
+    (4096, 8192, None, None, 1 << 17, (15, 22)), (4096, 8192, None, None, 1 << 17, (-32, 8))])
+def test_conv_refuses_shared_memory(x, w, state, lengths, out, ldo):
+    """x (2, 4, 8) float32, weight (8, 4): out or state over an input, over each other or over itself."""
+    assert status("tesm_b200_causal_conv", vp(x), 0, 32, 8, 2, 4, 8, 4, vp(w), None, vp(state), vp(lengths), 1, vp(out), *ldo,
+                  None) == 1
+    assert "causal_conv" in _lib.last_error()
+
+
+@pytest.mark.parametrize("which", ["x", "dt", "bm", "cm", "z", "A", "skip", "bias", "lengths", "state", "self", "negative"])
+@pytest.mark.parametrize("written", ["out", "state"])
+def test_scan_refuses_shared_memory(which, written):
+    at = {n: (i + 1) << 16 for i, n in enumerate(["x", "dt", "bm", "cm", "z", "out", "A", "skip", "bias", "state", "lengths"])}
+    s = [32, 8] * 2 + [64, 16] * 2 + [32, 8] * 2
+    if which == "self":
+        s[10] = 24
+    elif which == "negative":
+        s[1] = -8
+    elif which == "state":
+        at["out"] = at["state"] + 4
+    else:
+        at[written] = at[which] + 4
+    t = (ctypes.c_int64 * 12)(*s)
+    assert status("tesm_b200_ssm_scan", *(vp(at[n]) for n in ("x", "dt", "bm", "cm", "z", "out")), ctypes.addressof(t), 0, 2, 4,
+                  8, 16, vp(at["A"]), vp(at["skip"]), vp(at["bias"]), 1, vp(at["state"]), vp(at["lengths"]), None) == 1
 
 
 def test_cpu_tensors_are_refused():

@@ -158,13 +158,15 @@ def test_conv_refusals():
         with pytest.raises(ValueError):
             ops.causal_conv(*a)
     for kw in [dict(state=st.bfloat16()), dict(state=st[:, :2]), dict(lengths=torch.zeros(2, device="cuda")),
-               dict(out=x), dict(out=torch.zeros(2, 5, 7, device="cuda")), dict(out=x.bfloat16()),
-               dict(out=torch.zeros(1, 5, 8, device="cuda").expand(2, 5, 8)),
+               dict(out=torch.zeros(2, 5, 7, device="cuda")), dict(out=x.bfloat16()),
                dict(lengths=torch.zeros(3, dtype=torch.int32, device="cuda"))]:
         with pytest.raises(ValueError):
             ops.causal_conv(x, w, **kw)
     both = torch.zeros(2 * 5 * 8 + 48, device="cuda")
-    with pytest.raises(ValueError):
+    for kw in [dict(out=x), dict(out=torch.zeros(1, 5, 8, device="cuda").expand(2, 5, 8))]:
+        with pytest.raises(_lib.TesmError):
+            ops.causal_conv(x, w, **kw)
+    with pytest.raises(_lib.TesmError):
         ops.causal_conv(both[:80].view(2, 5, 8), w, state=both[60:108].view(2, 3, 8))
     with pytest.raises(_lib.TesmError):
         ops.causal_conv(x.half(), w)
@@ -407,10 +409,12 @@ def test_scan_refusals():
                       ("A", z(4)), ("A", z(4, 0)), ("A", z(4, 129)), ("A", z(8, 4).t()), ("A", z(4, 8).double()),
                       ("Bm", z(2, 5, 7)), ("Cm", z(2, 8, 5).transpose(1, 2)), ("D", z(5)), ("z", z(2, 4, 5).transpose(1, 2)),
                       ("dt_bias", z(8)[::2]), ("state", z(2, 4, 8).double()), ("state", z(2, 8, 4).transpose(1, 2)),
-                      ("state", z(1, 4, 8).expand(2, 4, 8)), ("lengths", z(2)), ("out", good["x"]), ("out", good["z"]),
-                      ("out", z(1, 5, 4).expand(2, 5, 4)), ("out", z(2, 5, 4).bfloat16())]:
+                      ("state", z(1, 4, 8).expand(2, 4, 8)), ("lengths", z(2)), ("out", z(2, 5, 4).bfloat16())]:
         with pytest.raises(ValueError):
             call({**good, name: bad})
+    for bad in (good["x"], good["z"], z(1, 5, 4).expand(2, 5, 4)):
+        with pytest.raises(_lib.TesmError):
+            call({**good, "out": bad})
     with pytest.raises(_lib.TesmError):
         call({**good, "x": good["x"].half()})
     with torch.enable_grad(), pytest.raises(RuntimeError):
