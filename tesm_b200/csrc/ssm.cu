@@ -7,6 +7,12 @@ namespace tesm {
 // x * sigmoid(x); 0 for x -> -inf (the reciprocal of inf is 0, and x * 0 stays finite for finite x)
 __device__ __forceinline__ float silu(float x) { return x * rcp_approx(1.f + ex2_approx(-x * kLog2e)); }
 
+__device__ __forceinline__ float2 silu2(float2 x) {
+  const float2 t = __fmul2_rn(x, make_float2(-kLog2e, -kLog2e));
+  const float2 d = __fadd2_rn(make_float2(ex2_approx(t.x), ex2_approx(t.y)), make_float2(1.f, 1.f));
+  return __fmul2_rn(x, make_float2(rcp_approx(d.x), rcp_approx(d.y)));
+}
+
 // softplus(x) = max(x, 0) + log(1 + u), u = e^-|x| in (0, 1].  log(1 + u) = 2 atanh(s) with
 // s = u / (2 + u) <= 1/3: the odd series in s keeps full relative accuracy for small u, where
 // forming 1 + u would round u away.  Terms to s^15 leave 1.4e-9 relative at s = 1/3.
@@ -40,7 +46,7 @@ __device__ __forceinline__ __nv_bfloat16 from_f(float x) { return __float2bfloat
 // N consecutive elements as they are in memory: one 16-byte access per 16 bytes where `vec`
 // promises alignment and all N exist, else the first `have` of them one by one (the rest zero).
 template <class T, int N>
-struct Pack {
+struct alignas(N * sizeof(T) >= 16 ? 16 : N * sizeof(T)) Pack {
   T v[N];
   __device__ __forceinline__ void load(const T *p, bool vec, int have) {
     if constexpr (N * sizeof(T) % 16 == 0) {
@@ -53,6 +59,12 @@ struct Pack {
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = i < have ? p[i] : from_f<T>(0.f);
+  }
+  __device__ __forceinline__ void load_all(const T *p) {  // 8 or 16 bytes, aligned
+    if constexpr (N * sizeof(T) == 8)
+      *reinterpret_cast<uint2 *>(v) = *reinterpret_cast<const uint2 *>(p);
+    else
+      *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(p);
   }
   __device__ __forceinline__ void store(T *p, bool vec, int have) const {
     if constexpr (N * sizeof(T) % 16 == 0) {
@@ -70,6 +82,10 @@ struct Pack {
   __device__ __forceinline__ void zero() {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = from_f<T>(0.f);
+  }
+  __device__ __forceinline__ void pairs(float2 (&f)[(N + 1) / 2]) const {
+#pragma unroll
+    for (int i = 0; i < (N + 1) / 2; ++i) f[i] = make_float2(to_f(v[2 * i]), 2 * i + 1 < N ? to_f(v[(2 * i + 1) % N]) : 0.f);
   }
 };
 
@@ -105,85 +121,139 @@ static bool self_overlap(int64_t B, int64_t L, int64_t n, int64_t ldb, int64_t l
 }
 
 // ------------------------------------------------------------ causal convolution
-// y_t = act(bias + sum_j w_j x_{t-K+1+j}).  A thread owns N channels (16 bytes of them) and walks
-// a tile of tokens with the last K - 1 inputs in registers, so x is read once (and K - 1 rows
-// again per tile) and y written once.
-constexpr int kConvThreads = 128;
+// y_t = act(bias + sum_j w_j x_{t-K+1+j}).  Bytes bound it: x is read once (and K - 1 rows again per
+// tile of tokens), y written once.  A thread owns N channels (16 bytes of them) and walks a tile
+// with the last K - 1 inputs in registers, two channels per packed FMA.  16 rows ahead are on
+// their way into the thread's own slots of shared memory: registers for as many would halve the
+// occupancy (4 rows ahead in registers: 116 us against 91 us, 5.9 TB/s, at 4 x 4096 tokens of 8192
+// bf16 channels, K = 4; a plain copy of the same bytes takes 87 us).  Rows are addressed by running
+// pointers, since 64-bit products per row cost as much as the arithmetic.  Single tokens take kConvBatch
+// sequences per thread, so that the weights are read less often (256 sequences: 11 us, against 18 with one).
+constexpr int kConvThreads = 128, kConvBatch = 4;
 
-template <class T, int N, int K>
+template <class T, int N, int K, int U>
 __global__ void __launch_bounds__(kConvThreads)
-    k_causal_conv(Rows<const T> x, int L, int D, int TT, int vec, const float *__restrict__ weight,
+    k_causal_conv(Rows<const T> x, int B, int L, int D, int TT, int nb, int vec, const float *__restrict__ weight,
                   const float *__restrict__ bias, T *__restrict__ state, const int *__restrict__ lengths, int act,
                   Rows<T> y, int chunks, int tiles) {
   pdl_trigger();
   pdl_wait();
   const int chunk = blockIdx.x % chunks;
   const int tile = blockIdx.x / chunks % tiles;
-  const int64_t b = blockIdx.x / chunks / tiles;
+  const int b0 = blockIdx.x / chunks / tiles * nb, b1 = min(b0 + nb, B);
   const int c = (chunk * kConvThreads + threadIdx.x) * N;
   if (c >= D) return;
   const int have = min(N, D - c);
-  const int T_b = seq_len(lengths, b, L);
-  T *st = state ? state + (b * (K - 1)) * D + c : nullptr;
-  // the input of position p >= 1 - K; before the start the state's rows
-  auto load = [&](Pack<T, N> &q, int p) {
-    if (p >= 0)
-      q.load(x.at(b, p, c), vec, have);
-    else if (st)
-      q.load(st + (int64_t)(p + K - 1) * D, vec, have);
-    else
-      q.zero();
-  };
-  const int t0 = tile * TT, t1 = min(t0 + TT, L), te = min(t1, T_b);
-  if (t0 < te) {
-    float w[K][N], bs[N], win[K][N];
+  constexpr bool kAsync = N * sizeof(T) == 16 && U > 1;
+  constexpr int kGroups = 8;  // groups of U rows in shared memory
+  __shared__ __align__(16) char smem[kAsync ? kGroups * U * kConvThreads * 16 : 16];
+  const uint32_t slot = (uint32_t)__cvta_generic_to_shared(smem) + threadIdx.x * 16;
+  constexpr int H2 = (N + 1) / 2;
+  float2 w[H2][K], bs[H2];  // pairs of channels, for packed arithmetic
+  {
+    float wf[2 * H2 * K];  // as in memory: channel by channel
+    if (N > 1 && have == N && ((uintptr_t)weight & 15) == 0) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      bs[e] = bias && e < have ? bias[c + e] : 0.f;
+      for (int i = 0; i < N * K / 4; ++i)
+        reinterpret_cast<float4 *>(wf)[i] = __ldg(reinterpret_cast<const float4 *>(weight + (int64_t)c * K) + i);
+    } else {
 #pragma unroll
-      for (int j = 0; j < K; ++j) w[j][e] = e < have ? weight[(int64_t)(c + e) * K + j] : 0.f;
+      for (int i = 0; i < 2 * H2 * K; ++i) wf[i] = i / K < have ? weight[(int64_t)c * K + i] : 0.f;
     }
 #pragma unroll
-    for (int j = 0; j < K - 1; ++j) {
-      Pack<T, N> q;
-      load(q, t0 - (K - 1) + j);
+    for (int h = 0; h < H2; ++h) {
+      bs[h] = make_float2(bias && 2 * h < have ? bias[c + 2 * h] : 0.f, bias && 2 * h + 1 < have ? bias[c + 2 * h + 1] : 0.f);
 #pragma unroll
-      for (int e = 0; e < N; ++e) win[j][e] = to_f(q.v[e]);
-    }
-    constexpr int U = 4;  // rows loaded ahead of their use
-    for (int t = t0; t < te; t += U) {
-      Pack<T, N> in[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (t + u < te) in[u].load(x.at(b, t + u, c), vec, have);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (t + u >= te) break;
-        Pack<T, N> out;
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-          win[K - 1][e] = to_f(in[u].v[e]);
-          float acc = bs[e];
-#pragma unroll
-          for (int j = 0; j < K; ++j) acc = fmaf(w[j][e], win[j][e], acc);
-          out.v[e] = from_f<T>(act ? silu(acc) : acc);
-#pragma unroll
-          for (int j = 0; j < K - 1; ++j) win[j][e] = win[j + 1][e];
-        }
-        out.store(y.at(b, t + u, c), vec, have);
-      }
+      for (int j = 0; j < K; ++j) w[h][j] = make_float2(wf[2 * h * K + j], wf[(2 * h + 1) * K + j]);
     }
   }
-  Pack<T, N> z;
-  z.zero();
-  for (int t = max(t0, te); t < t1; ++t) z.store(y.at(b, t, c), vec, have);
-  // only the first tile reads the state, so the thread that has read it may replace it
-  if (tile == 0 && st && T_b > 0) {
-    Pack<T, N> q[K - 1];
+  const int t0 = tile * TT, t1 = min(t0 + TT, L);
+  Pack<T, N> zero;
+  zero.zero();
+  for (int b = b0; b < b1; ++b) {
+    const int T_b = seq_len(lengths, b, L), te = min(t1, T_b);
+    T *st = state ? state + (int64_t)b * (K - 1) * D + c : nullptr;
+    // the input of position p >= 1 - K; before the start the state's rows
+    auto load = [&](Pack<T, N> &q, int p) {
+      if (p >= 0)
+        q.load(x.at(b, p, c), vec, have);
+      else if (st)
+        q.load(st + (int64_t)(p + K - 1) * D, vec, have);
+      else
+        q.zero();
+    };
+    if (t0 < te) {
+      constexpr int H = (N + 1) / 2;
+      Pack<T, N> first[K - 1], next[U];
+      // rows [t, t + U) on their way: into this thread's own slots of shared memory (whole 16-byte
+      // accesses), or into registers
+      const T *xp = x.at(b, t0, c);  // the next row to request
+      T *yp = y.at(b, t0, c);        // the next row to store
+      auto request = [&](int t) {
 #pragma unroll
-    for (int j = 0; j < K - 1; ++j) load(q[j], T_b - (K - 1) + j);
+        for (int u = 0; u < U; ++u) {
+          if constexpr (kAsync) {
+            if (t + u < te)
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot + (uint32_t)(t + u - t0) % (kGroups * U) * (kConvThreads * 16)),
+                           "l"(xp) : "memory");
+          } else {
+            next[u].load(xp, vec, t + u < te ? have : 0);
+          }
+          xp += x.ldl;
+        }
+        if constexpr (kAsync) asm volatile("cp.async.commit_group;" ::: "memory");
+      };
 #pragma unroll
-    for (int j = 0; j < K - 1; ++j) q[j].store(st + (int64_t)j * D, vec, have);
+      for (int g = 0; g < (kAsync ? kGroups - 1 : 1); ++g) request(t0 + g * U);
+#pragma unroll
+      for (int j = 0; j < K - 1; ++j) load(first[j], t0 - (K - 1) + j);
+      float2 win[K - 1 + U][H];  // the last K - 1 inputs, then U new ones
+#pragma unroll
+      for (int j = 0; j < K - 1; ++j) first[j].pairs(win[j]);
+      for (int t = t0; t < te; t += U) {
+        if constexpr (kAsync) {
+          request(t + (kGroups - 1) * U);
+          asm volatile("cp.async.wait_group %0;" ::"n"(kGroups - 1) : "memory");
+#pragma unroll
+          for (int u = 0; u < U; ++u) {  // slots behind the end hold old rows: computed, not stored
+            Pack<T, N> q = *reinterpret_cast<const Pack<T, N> *>(smem + (uint32_t)(t + u - t0) % (kGroups * U) * (kConvThreads * 16) + threadIdx.x * 16);
+            q.pairs(win[K - 1 + u]);
+          }
+        } else {
+#pragma unroll
+          for (int u = 0; u < U; ++u) next[u].pairs(win[K - 1 + u]);
+          request(t + U);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          Pack<T, N> out;
+#pragma unroll
+          for (int h = 0; h < H; ++h) {
+            float2 acc = bs[h];
+#pragma unroll
+            for (int j = 0; j < K; ++j) acc = __ffma2_rn(w[h][j], win[u + j][h], acc);
+            if (act) acc = silu2(acc);
+            out.v[2 * h] = from_f<T>(acc.x);
+            if (2 * h + 1 < N) out.v[2 * h + 1] = from_f<T>(acc.y);
+          }
+          if (t + u < te) out.store(yp, vec, have);
+          yp += y.ldl;
+        }
+#pragma unroll
+        for (int j = 0; j < K - 1; ++j)
+#pragma unroll
+          for (int h = 0; h < H; ++h) win[j][h] = win[U + j][h];
+      }
+    }
+    for (int t = max(t0, te); t < t1; ++t) zero.store(y.at(b, t, c), vec, have);
+    // only the first tile reads the state, so the thread that has read it may replace it
+    if (tile == 0 && st && T_b > 0) {
+      Pack<T, N> q[K - 1];
+#pragma unroll
+      for (int j = 0; j < K - 1; ++j) load(q[j], T_b - (K - 1) + j);
+#pragma unroll
+      for (int j = 0; j < K - 1; ++j) q[j].store(st + (int64_t)j * D, vec, have);
+    }
   }
 }
 
@@ -353,52 +423,143 @@ __global__ void __launch_bounds__(kScanThreads) k_ssm_scan(const __grid_constant
 
 // ------------------------------------------------------------ selective scan, single tokens
 // One token per sequence: the state is read and written once, which bounds it.  LPC lanes of 4
-// states per channel; a thread keeps its row of A for kStepBatch sequences.
-constexpr int kStepThreads = 256, kStepBatch = 8;
+// states per channel; a thread keeps its row of A for kStepBatch sequences and takes R of them at
+// a time: lane q of a channel forms softplus, dt * x and the gate of sequence q % R, the others
+// get them by shuffles, and the sums over the states end in that lane again (transposed
+// reduction).  With VEC (N a multiple of 4, aligned rows) the states of the next kStepAhead - 1
+// groups are on their way into the thread's own slots of shared memory, and the next group's
+// inputs into registers, while one group is computed.
+constexpr int kStepThreads = 128, kStepAhead = 2, kStepBatch = 16;
 
-template <class T, bool VEC>
-__global__ void __launch_bounds__(kStepThreads)
-    k_ssm_step(const __grid_constant__ ScanArgs<T> a, int B, int lpc) {
+template <class T, bool VEC, int LPC>
+__global__ void __launch_bounds__(kStepThreads, 5) k_ssm_step(const __grid_constant__ ScanArgs<T> a, int B) {
+  constexpr int R = LPC < 4 ? LPC : 4;
+  __shared__ __align__(16) char smem[VEC ? kStepAhead * R * kStepThreads * 16 : 16];
   pdl_trigger();
   pdl_wait();
-  const int per = kStepThreads / lpc;
-  const int q = threadIdx.x % lpc, n0 = q * 4;
-  const int c = (int)(blockIdx.x % a.chunks) * per + threadIdx.x / lpc;
+  const int q = threadIdx.x % LPC, n0 = q * 4, my = q % R;
+  const int c = (int)(blockIdx.x % a.chunks) * (kStepThreads / LPC) + threadIdx.x / LPC;
   const int b0 = (int)(blockIdx.x / a.chunks) * kStepBatch, b1 = min(b0 + kStepBatch, B);
   const bool live = c < a.D;
   const int have = live ? min(4, a.N - n0) : 0;
+  // four states, or inputs of them: with VEC all or none of them exist
+  auto load4 = [&](auto &p, const auto *src, bool on) {
+    if constexpr (VEC) {
+      p.zero();
+      if (on && have > 0) p.load_all(src);
+    } else {
+      p.load(src, false, on ? have : 0);
+    }
+  };
   Pack<float, 4> A;
-  A.load(a.A + (int64_t)c * a.N + n0, VEC, have);
+  load4(A, a.A + (int64_t)c * a.N + n0, true);
 #pragma unroll
   for (int i = 0; i < 4; ++i) A.v[i] *= kLog2e;
   const float bias = live && a.dt_bias ? a.dt_bias[c] : 0.f, skip = live && a.skip ? a.skip[c] : 0.f;
-#pragma unroll 2
-  for (int b = b0; b < b1; ++b) {
-    const bool on = live && seq_len(a.lengths, b, 1) > 0;
-    const int hv = on ? have : 0;
-    Pack<float, 4> h;
-    h.zero();
-    float *st = a.state ? a.state + ((int64_t)b * a.D + c) * a.N + n0 : nullptr;
-    if (st) h.load(st, VEC, hv);
-    Pack<T, 4> bm, cm;
-    bm.load(a.bm.at(b, 0, n0), false, hv);
-    cm.load(a.cm.at(b, 0, n0), false, hv);
-    const float x = on ? to_f(*a.x.at(b, 0, c)) : 0.f;
-    float d = on ? to_f(*a.dt.at(b, 0, c)) + bias : 0.f;
-    if (a.softplus) d = softplus(d);
-    float y = 0.f;
+  const int64_t row = (int64_t)a.D * a.N;
+  float *st = a.state ? a.state + b0 * row + (int64_t)c * a.N + n0 : nullptr;
+  const float *ahead = st;  // the next state to request
+  const uint32_t slot = (uint32_t)__cvta_generic_to_shared(smem) + threadIdx.x * 16;
+  int ring = 0;  // the group of slots requested next
+  auto request = [&](int b) {
+    if constexpr (VEC) {
+      if (st && have > 0) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      h.v[i] = fmaf(ex2_approx(d * A.v[i]), h.v[i], d * x * to_f(bm.v[i]));
-      y = fmaf(to_f(cm.v[i]), h.v[i], y);
+        for (int r = 0; r < R; ++r) {
+          if (b + r < b1)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot + (ring * R + r) * (kStepThreads * 16)),
+                         "l"(ahead) : "memory");
+          ahead += row;
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      ring = ring + 1 == kStepAhead ? 0 : ring + 1;
     }
-    if (st) h.store(st, VEC, hv);
-    for (int o = lpc / 2; o; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-    if (q == 0 && live) {
-      y = fmaf(skip, x, y);
-      if (a.z.p && on) y *= silu(to_f(*a.z.at(b, 0, c)));
-      *a.out.at(b, 0, c) = from_f<T>(on ? y : 0.f);
+  };
+  const T *px = a.x.at(b0 + my, 0, c), *pd = a.dt.at(b0 + my, 0, c), *pz = a.z.p ? a.z.at(b0 + my, 0, c) : nullptr;
+  const T *pb = a.bm.at(b0, 0, n0), *pc = a.cm.at(b0, 0, n0);
+  T *po = a.out.at(b0 + my, 0, c);
+  struct In {
+    Pack<T, 4> bm[R], cm[R];
+    T x, d, z;
+    bool on;  // this lane's sequence has a token
+  } next;
+  auto fetch = [&](In &in, int b) {  // sequences b .. b + R - 1; b rises by R from call to call
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      load4(in.bm[r], pb, b + r < b1);
+      load4(in.cm[r], pc, b + r < b1);
+      pb += a.bm.ldb, pc += a.cm.ldb;
     }
+    in.on = live && b + my < b1 && (!a.lengths || a.lengths[b + my] > 0);
+    in.x = in.on ? *px : from_f<T>(0.f);
+    in.d = in.on ? *pd : from_f<T>(0.f);
+    in.z = in.on && pz ? *pz : from_f<T>(0.f);
+    px += R * a.x.ldb, pd += R * a.dt.ldb;
+    if (pz) pz += R * a.z.ldb;
+  };
+#pragma unroll
+  for (int k = 0; k < kStepAhead - 1; ++k) request(b0 + k * R);
+  fetch(next, b0);
+  int used = 0;  // the group of slots read next
+  for (int b = b0; b < b1; b += R) {
+    request(b + (kStepAhead - 1) * R);
+    const In in = next;
+    fetch(next, b + R);
+    float d = to_f(in.d) + bias;
+    if (a.softplus) d = softplus(d);
+    if (!in.on) d = 0.f;
+    const float u = d * to_f(in.x);
+    if constexpr (VEC) asm volatile("cp.async.wait_group %0;" ::"n"(kStepAhead - 1) : "memory");
+    float y[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      Pack<float, 4> h;
+      if constexpr (VEC) {
+        h.zero();
+        if (st && have > 0 && b + r < b1)
+          h.load_all(reinterpret_cast<const float *>(smem + (used * R + r) * (kStepThreads * 16) + threadIdx.x * 16));
+      } else {
+        h.load(st, false, st && b + r < b1 ? have : 0);
+      }
+      const float dr = __shfl_sync(0xffffffffu, d, r, R), ur = __shfl_sync(0xffffffffu, u, r, R);
+      const bool on = __shfl_sync(0xffffffffu, in.on, r, R);
+      y[r] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // a sequence without a token may hold anything in its row of B and C
+        h.v[i] = fmaf(ex2_approx(dr * A.v[i]), h.v[i], ur * to_f(in.bm[r].v[i]));
+        y[r] = fmaf(to_f(in.cm[r].v[i]), h.v[i], y[r]);
+      }
+      if (st) {
+        if (on) {
+          if constexpr (VEC) {
+            if (have > 0) *reinterpret_cast<float4 *>(st) = *reinterpret_cast<const float4 *>(h.v);
+          } else {
+            h.store(st, false, have);
+          }
+        }
+        st += row;
+      }
+    }
+    used = used + 1 == kStepAhead ? 0 : used + 1;
+#pragma unroll
+    for (int o = R / 2; o; o >>= 1) {
+#pragma unroll
+      for (int j = 0; j < o; ++j) {
+        const bool up = q & o;
+        const float keep = up ? y[j + o] : y[j], give = up ? y[j] : y[j + o];
+        y[j] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+      }
+    }
+#pragma unroll
+    for (int o = R; o < LPC; o <<= 1) y[0] += __shfl_xor_sync(0xffffffffu, y[0], o);
+    if (q < R && live && b + my < b1) {
+      float o = fmaf(skip, to_f(in.x), y[0]);
+      if (a.z.p) o *= silu(to_f(in.z));
+      *po = from_f<T>(in.on ? o : 0.f);
+    }
+    po += R * a.out.ldb;
   }
 }
 
@@ -426,17 +587,28 @@ static int launch_scan_lanes(const ScanArgs<T> &a, int64_t B, int lpc, cudaStrea
   }
 }
 
+template <class T, int LPC>
+static int launch_step(ScanArgs<T> a, int64_t B, cudaStream_t st) {
+  a.chunks = (int)ceil_div(a.D, kStepThreads / LPC);
+  const dim3 grid((unsigned)(a.chunks * ceil_div(B, kStepBatch))), block(kStepThreads);
+  const bool vec = a.N % 4 == 0 && a.vec_bc && (((uintptr_t)a.A | (uintptr_t)a.state) & 15) == 0;
+  return vec ? launch_k("ssm_scan", k_ssm_step<T, true, LPC>, grid, block, 0, st, a, (int)B)
+             : launch_k("ssm_scan", k_ssm_step<T, false, LPC>, grid, block, 0, st, a, (int)B);
+}
+
 template <class T>
 static int ssm_scan_t(ScanArgs<T> a, int64_t B, cudaStream_t st) {
   int np = 1;
   while (np < a.N) np <<= 1;
   if (a.L == 1) {
-    const int lpc = np <= 4 ? 1 : np / 4;
-    a.chunks = (int)ceil_div(a.D, kStepThreads / lpc);
-    const dim3 grid((unsigned)(a.chunks * ceil_div(B, kStepBatch))), block(kStepThreads);
-    const bool vec = a.N % 4 == 0 && (((uintptr_t)a.A | (uintptr_t)a.state) & 15) == 0;
-    return vec ? launch_k("ssm_scan", k_ssm_step<T, true>, grid, block, 0, st, a, (int)B, lpc)
-               : launch_k("ssm_scan", k_ssm_step<T, false>, grid, block, 0, st, a, (int)B, lpc);
+    switch (np <= 4 ? 1 : np / 4) {
+      case 1: return launch_step<T, 1>(a, B, st);
+      case 2: return launch_step<T, 2>(a, B, st);
+      case 4: return launch_step<T, 4>(a, B, st);
+      case 8: return launch_step<T, 8>(a, B, st);
+      case 16: return launch_step<T, 16>(a, B, st);
+      default: return launch_step<T, 32>(a, B, st);
+    }
   }
   // States per lane: as many as still give every SM a block; fewer states per lane spread a
   // channel over more lanes.
@@ -448,18 +620,20 @@ static int ssm_scan_t(ScanArgs<T> a, int64_t B, cudaStream_t st) {
                     : launch_scan_lanes<T, 1>(a, B, lpc, st);
 }
 
-template <class T, int N>
+template <class T, int N, int U>
 static int launch_conv(Rows<const T> x, int64_t B, int L, int D, int K, int vec, const float *w, const float *bias,
                        T *state, const int *lengths, int act, Rows<T> y, cudaStream_t st) {
   const int chunks = (int)ceil_div(D, kConvThreads * N);
   int TT = 64;  // tokens per tile: shorter while the blocks do not fill the SMs
   while (TT > 8 && B * chunks * ceil_div(L, TT) < 8 * (int64_t)sm_count()) TT >>= 1;
   const int tiles = (int)ceil_div(L, TT);
-  const dim3 grid((unsigned)(B * chunks * tiles)), block(kConvThreads);
+  // sequences per thread: several where a tile is short, so that the weights are loaded less often
+  const int nb = L < 4 && B * chunks >= kConvBatch * 2 * (int64_t)sm_count() ? kConvBatch : 1;
+  const dim3 grid((unsigned)(ceil_div(B, nb) * chunks * tiles)), block(kConvThreads);
 #define TESM_CONV(KK)                                                                                            \
   case KK:                                                                                                       \
-    return launch_k("causal_conv", k_causal_conv<T, N, KK>, grid, block, 0, st, x, L, D, TT, vec, w, bias, state, \
-                    lengths, act, y, chunks, tiles)
+    return launch_k("causal_conv", k_causal_conv<T, N, KK, U>, grid, block, 0, st, x, (int)B, L, D, TT, nb, vec, w, bias, \
+                    state, lengths, act, y, chunks, tiles)
   switch (K) {
     TESM_CONV(2);
     TESM_CONV(3);
@@ -482,9 +656,11 @@ static int causal_conv_t(const void *x, int64_t ldb, int64_t ldl, int64_t B, int
   const uint64_t bits = (uintptr_t)x | (uintptr_t)y | (uintptr_t)state |
                         (uint64_t)((ldb | ldl | ldyb | ldyl | (state ? D : 0)) * (int64_t)sizeof(T));
   constexpr int N = 16 / sizeof(T);
+  if (bits % 16 == 0 && L >= 4)
+    return launch_conv<T, N, 2>(rx, B, (int)L, (int)D, (int)K, 1, w, bias, (T *)state, lengths, act, ry, st);
   if (bits % 16 == 0)
-    return launch_conv<T, N>(rx, B, (int)L, (int)D, (int)K, 1, w, bias, (T *)state, lengths, act, ry, st);
-  return launch_conv<T, 1>(rx, B, (int)L, (int)D, (int)K, 0, w, bias, (T *)state, lengths, act, ry, st);
+    return launch_conv<T, N, 1>(rx, B, (int)L, (int)D, (int)K, 1, w, bias, (T *)state, lengths, act, ry, st);
+  return launch_conv<T, 1, 4>(rx, B, (int)L, (int)D, (int)K, 0, w, bias, (T *)state, lengths, act, ry, st);
 }
 
 }  // namespace tesm
