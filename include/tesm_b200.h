@@ -345,7 +345,7 @@ int tesm_b200_siso_scan_noalloc(const void *proj, int dtype, int64_t ldp, int64_
  * as the largest finite float.  finished and lengths are nullable (none finished; lengths 0, only
  * with length_penalty == 0).  1 <= W, K <= 32.  Two launches; ws: 16-byte aligned scratch of
  * tesm_b200_beam_select_workspace bytes, free again once the work has run on the stream. */
-int tesm_b200_beam_select_workspace(int64_t G, int64_t W, int64_t V, int64_t K, int64_t *bytes_out);
+int tesm_b200_beam_select_workspace(int dtype, int64_t G, int64_t W, int64_t V, int64_t K, int64_t *bytes_out);
 int tesm_b200_beam_select(const void *logits, int dtype, int64_t ldg, int64_t ldw, int64_t G, int64_t W, int64_t V,
                           int64_t K, const float *scores, const uint8_t *finished, const int32_t *lengths,
                           int64_t eos, int64_t pad, double length_penalty, int64_t *tokens, int32_t *parents,

@@ -81,7 +81,7 @@ SIGNATURES = {
                                  c_vp, c_i64, c_vp],
     "tesm_b200_siso_scan_noalloc": [c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp,
                                     c_vp, c_vp, c_vp, c_vp],
-    "tesm_b200_beam_select_workspace": [c_i64, c_i64, c_i64, c_i64, c_vp],
+    "tesm_b200_beam_select_workspace": [c_int, c_i64, c_i64, c_i64, c_i64, c_vp],
     "tesm_b200_beam_select": [c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_i64, c_i64,
                               c_double, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp],
     "tesm_b200_reorder_states": [c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp],

@@ -547,9 +547,9 @@ class BeamStep:
 
 
 @lru_cache(maxsize=256)
-def _beam_workspace(G: int, W: int, V: int, K: int) -> int:
+def _beam_workspace(dtype: int, G: int, W: int, V: int, K: int) -> int:
     n = ctypes.c_int64(0)
-    _lib.call("tesm_b200_beam_select_workspace", G, W, V, K, ctypes.addressof(n))
+    _lib.call("tesm_b200_beam_select_workspace", dtype, G, W, V, K, ctypes.addressof(n))
     return n.value
 
 
@@ -591,7 +591,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: Optional[int]
     out_scores = scores.new_empty(out)
     out_finished = scores.new_empty(out, dtype=torch.bool)
     out_lengths = scores.new_empty(out, dtype=torch.int32)
-    ws_bytes = _beam_workspace(G, W, V, K)
+    ws_bytes = _beam_workspace(code, G, W, V, K)
     ws = scores.new_empty(ws_bytes, dtype=torch.uint8)
     _call_on(dev, "tesm_b200_beam_select", logits.data_ptr(), code, ldg if G > 1 else 0, ldw if W > 1 else 0, G, W, V,
              K, scores.data_ptr(), _ptr(finished), _ptr(lengths), -1 if eos_token_id is None else eos_token_id,

@@ -31,10 +31,10 @@ def test_beam_select_refuses(kw, want):
 
 def test_beam_workspace():
     n = ctypes.c_int64(-1)
-    assert status("tesm_b200_beam_select_workspace", 2, 4, 32000, 4, ctypes.addressof(n)) == 0 and n.value > 0
-    assert status("tesm_b200_beam_select_workspace", 0, 4, 32000, 4, ctypes.addressof(n)) == 0 and n.value == 0
-    assert status("tesm_b200_beam_select_workspace", 2, 33, 32000, 4, ctypes.addressof(n)) == 1
-    assert status("tesm_b200_beam_select_workspace", 2, 4, 32000, 4, None) == 1
+    assert status("tesm_b200_beam_select_workspace", 0, 2, 4, 32000, 4, ctypes.addressof(n)) == 0 and n.value > 0
+    assert status("tesm_b200_beam_select_workspace", 1, 0, 4, 32000, 4, ctypes.addressof(n)) == 0 and n.value == 0
+    assert status("tesm_b200_beam_select_workspace", 0, 2, 33, 32000, 4, ctypes.addressof(n)) == 1
+    assert status("tesm_b200_beam_select_workspace", 0, 2, 4, 32000, 4, None) == 1
 
 
 def rows(*entries):
