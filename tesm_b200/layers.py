@@ -752,3 +752,79 @@ def generate(lm, input_ids, max_new_tokens=64, temperature=1.0, top_k=0, use_cac
             out, _ = lm(generated[:, -cfg.max_seq_len:])
             logits = out.logits[:, -1, :]
     return generated
+
+
+@torch.no_grad()
+def beam_search(lm, input_ids, num_beams=4, max_new_tokens=64, length_penalty=1.0, num_return_sequences=1,
+                use_graph=None):
+    """Beam search with the recurrent-state cache: one prefill per prompt, its caches spread over the
+    beams, then per token one decode step of all beams, the selection (``ops.beam_select``) and the
+    caches following their beams (``ops.StateReorder``, in place, so a captured decode graph keeps
+    its buffers).  Ended beams (``eos_token_id``) stay in the beam with their score; hypotheses are
+    ranked by summed log-probability / new tokens ** length_penalty, EOS counted.  Returns the
+    sequences (prompts, num_return_sequences, prompt + new tokens), padded with ``pad_token_id``
+    behind EOS, and their scores, best first; a prompt with fewer than that many hypotheses fills up
+    with scores of -inf."""
+    lm.eval()
+    cfg = lm.tesm_config
+    if input_ids.dim() != 2 or input_ids.shape[0] < 1 or input_ids.shape[1] < 1:
+        raise ValueError(f"beam_search needs prompts of shape (batch, tokens), got {tuple(input_ids.shape)}")
+    G, L = input_ids.shape
+    W, n_ret, steps = int(num_beams), int(num_return_sequences), int(max_new_tokens)
+    if not 1 <= W <= ops.MAX_BEAMS or not 1 <= n_ret <= W or steps < 1:
+        raise ValueError(f"beam_search needs 1 to {ops.MAX_BEAMS} beams, at most as many returned sequences and a new "
+                         f"token, got {W}, {n_ret}, {steps}")
+    if L + steps - 1 > cfg.max_seq_len:
+        raise ValueError(f"Sequence length {L + steps - 1} exceeds max_seq_len {cfg.max_seq_len}")
+    if not 0 <= cfg.pad_token_id < cfg.vocab_size:
+        raise ValueError(f"pad_token_id {cfg.pad_token_id} is outside the vocabulary of {cfg.vocab_size}")
+    first = lm.backbone.layers[0]
+    if parallel.get_tp(first.mlp) is not None or parallel.mixer_tp(first.mixer) is not None:
+        raise TesmError("tesm_b200: beam_search does not run on tensor-parallel layers")
+    eos = getattr(cfg, "eos_token_id", None)
+    pick = dict(eos_token_id=eos, pad_token_id=cfg.pad_token_id, length_penalty=float(length_penalty))
+    ip = {"state_cache": lm.backbone.allocate_inference_cache(G, cfg.max_seq_len)}
+    out, _ = lm(input_ids, inference_params=ip, logits_to_keep=1)
+    dev = out.logits.device
+    logits = out.logits[:, -1:, :]
+    step = ops.beam_select(logits, torch.zeros(G, 1, device=dev), W,
+                           lengths=torch.zeros(G, 1, device=dev, dtype=torch.int32), **pick)
+    seqs = torch.full((G * W, steps), cfg.pad_token_id, device=dev, dtype=torch.int64)
+    seqs[:, 0] = step.tokens.view(-1)
+    done = 1
+    if steps > 1:
+        names = ("state", "ent_k_cache", "ent_v_cache")
+        narrow, wide = ip["state_cache"], lm.backbone.allocate_inference_cache(G * W, cfg.max_seq_len)
+        for i, c in narrow.items():
+            _prepare_cache(wide[i], dev)
+            wide[i]["seq_pos"], wide[i]["cache_idx"] = c["seq_pos"], c["cache_idx"]
+            wide[i]["_b200_no_state_out"] = True
+        ops.reorder_states([c[n] for c in narrow.values() for n in names], step.parents,
+                           out=[c[n] for c in wide.values() for n in names])
+        ip = {"state_cache": wide}
+        reorder = ops.StateReorder([c[n] for c in wide.values() for n in names] + [seqs], W)
+        if use_graph is None:
+            use_graph = steps >= GRAPH_MIN_TOKENS
+        graph = None
+        for done in range(1, steps):
+            if eos is not None and bool(step.finished.all()):
+                break
+            tokens = step.tokens.view(-1, 1)
+            if use_graph:
+                if graph is None:
+                    graph = DecodeGraph(lm, ip, tokens, greedy=False)
+                logits = graph.step_logits(tokens)
+            else:
+                out, _ = lm(tokens, inference_params=ip)
+                logits = out.logits[:, -1, :]
+            step = ops.beam_select(logits.view(G, W, -1), step.scores, finished=step.finished, lengths=step.lengths,
+                                   **pick)
+            reorder(step.parents)
+            seqs[:, done] = step.tokens.view(-1)
+        else:
+            done = steps
+    scores = step.scores[:, :n_ret].double()
+    if length_penalty != 0.0:
+        scores = scores / step.lengths[:, :n_ret].clamp(min=1).double() ** float(length_penalty)
+    new = seqs.view(G, W, steps)[:, :n_ret, :done]
+    return torch.cat([input_ids[:, None, :].expand(-1, n_ret, -1), new], dim=2), scores.float()

@@ -221,6 +221,14 @@ class TESMLMHeadModel(nn.Module):
         path (this model raises for it), so they are accepted and have no effect."""
         return layers.generate(self, input_ids, max_new_tokens, temperature, top_k, use_cache, use_graph)
 
+    @torch.no_grad()
+    def beam_search(self, input_ids, num_beams: int = 4, max_new_tokens: int = 64, length_penalty: float = 1.0,
+                    num_return_sequences: int = 1, use_graph=None):
+        """Beam search over the recurrent-state cache: (sequences, scores), best first.  See
+        ``layers.beam_search``; the reference has no counterpart."""
+        return layers.beam_search(self, input_ids, num_beams, max_new_tokens, length_penalty, num_return_sequences,
+                                  use_graph)
+
 
 def _init_weights(module, n_layer, initializer_range=0.02, rescale_prenorm_residual=True, n_residuals_per_layer=1):
     """Seeded init of mixer_seq_simple.py:790-803.
