@@ -15,19 +15,31 @@ __device__ __forceinline__ float2 silu2(float2 x) {
 
 // softplus(x) = max(x, 0) + log(1 + u), u = e^-|x| in (0, 1].  log(1 + u) = 2 atanh(s) with
 // s = u / (2 + u) <= 1/3: the odd series in s keeps full relative accuracy for small u, where
-// forming 1 + u would round u away.  Terms to s^15 leave 1.4e-9 relative at s = 1/3.
+// forming 1 + u would round u away.  Terms to s^13 leave 1.6e-8 relative at s = 1/3.
+__device__ __forceinline__ float2 softplus2(float2 x) {
+  const float2 u = make_float2(ex2_approx(-fabsf(x.x) * kLog2e), ex2_approx(-fabsf(x.y) * kLog2e));
+  const float2 den = __fadd2_rn(u, make_float2(2.f, 2.f));
+  const float2 s = __fmul2_rn(u, make_float2(rcp_approx(den.x), rcp_approx(den.y))), q = __fmul2_rn(s, s);
+  float2 p = make_float2(1.f / 13.f, 1.f / 13.f);
+  p = __ffma2_rn(p, q, make_float2(1.f / 11.f, 1.f / 11.f));
+  p = __ffma2_rn(p, q, make_float2(1.f / 9.f, 1.f / 9.f));
+  p = __ffma2_rn(p, q, make_float2(1.f / 7.f, 1.f / 7.f));
+  p = __ffma2_rn(p, q, make_float2(1.f / 5.f, 1.f / 5.f));
+  p = __ffma2_rn(p, q, make_float2(1.f / 3.f, 1.f / 3.f));
+  p = __ffma2_rn(p, q, make_float2(1.f, 1.f));
+  return __ffma2_rn(__fadd2_rn(s, s), p, make_float2(fmaxf(x.x, 0.f), fmaxf(x.y, 0.f)));
+}
 __device__ __forceinline__ float softplus(float x) {
   const float u = ex2_approx(-fabsf(x) * kLog2e);
   const float s = u * rcp_approx(2.f + u), q = s * s;
-  float p = 1.f / 15.f;
-  p = fmaf(p, q, 1.f / 13.f);
+  float p = 1.f / 13.f;
   p = fmaf(p, q, 1.f / 11.f);
   p = fmaf(p, q, 1.f / 9.f);
   p = fmaf(p, q, 1.f / 7.f);
   p = fmaf(p, q, 1.f / 5.f);
   p = fmaf(p, q, 1.f / 3.f);
   p = fmaf(p, q, 1.f);
-  return fmaxf(x, 0.f) + 2.f * s * p;
+  return fmaf(s + s, p, fmaxf(x, 0.f));
 }
 
 template <class T>
@@ -257,29 +269,22 @@ __global__ void __launch_bounds__(kConvThreads)
   }
 }
 
-// ------------------------------------------------------------ selective scan, prompts
+// ------------------------------------------------------------ selective scan, prompts: lanes share the states
 // h_t = exp(dt_t A) h_{t-1} + (dt_t x_t) B_t,  y_t = C_t . h_t + D x_t,  out = y silu(z).
-// A channel's N states are spread over LPC lanes with NPT states each (zero-padded to NPT * LPC);
-// a block of 128 threads walks the sequence of 128 / LPC channels in tiles of TT tokens.  Per
-// tile: softplus and dt * x are formed once per (token, channel) and staged in fp32 with B and
-// C; the raw rows of the next tile are loaded while this one is computed.  The sums over a
-// channel's lanes are transposed-reduced: LPC tokens' partial sums exchange halves in log2(LPC)
-// rounds, so that a token costs one shuffle instead of log2(LPC).
-constexpr int kScanThreads = 128;
-
-template <int NPT, int LPC>
-struct ScanShape {
-  static constexpr int NP = NPT * LPC;             // padded states per channel
-  static constexpr int CT = kScanThreads / LPC;    // channels per block
-  static constexpr int TT = LPC >= 32 ? 32 : LPC >= 8 ? 64 : 1024 / CT;  // tokens per tile
-  static constexpr int V = CT >= 8 ? 8 : 4;        // channels per row access
-  static constexpr int ITEMS = TT * CT / V;        // row accesses per tile and tensor (<= threads)
-  static constexpr int BV = NP >= 8 ? 8 : NP;      // states per access of B and C
-  static constexpr int BITEMS = TT * (NP / BV);
-  static constexpr int BIPT = (BITEMS + kScanThreads - 1) / kScanThreads;
-  static constexpr int SMEM = (TT * CT * 3 + 2 * TT * NP) * 4;
-};
-
+// A channel's N states are spread over LPC lanes with NPT states each (zero-padded to NPT * LPC),
+// which walk the sequence in double groups of 2 LPC tokens.  Lane q loads tokens q and LPC + q of
+// a group straight from the rows of x, dt and z (any alignment; kScanAhead tokens before their
+// use), forms softplus and dt * x for both in packed arithmetic and hands them to the others by
+// shuffles; the sums over the states end in the token's lane again (transposed reduction: LPC
+// partial sums exchange halves in log2(LPC) rounds), which gates and stores it.  So the
+// per-channel work is done once, and only B and C, shared by all channels, go through shared
+// memory, in fp32 tiles of 64 tokens.
+// Bytes do not bound it (41 us for one bf16 prompt of 4096 tokens, 8192 channels, 16 states), nor
+// the 20 exponentials and reciprocals per token and channel (149 us at 16 a clock and SM), but the 11
+// instructions per state at the issue rate of the 7 warps an SM gets from one sequence: 340 us; four
+// sequences of 2048 tokens, twice the work, take 506 us.
+// Inputs staged through shared memory with softplus formed by the loading thread took 354 us; 16 instead of
+// 32 tokens ahead 368 us; two states per lane (twice the warps, 16 instructions per state) 541 us.
 template <class T>
 struct ScanArgs {
   Rows<const T> x, dt, bm, cm, z;
@@ -290,76 +295,80 @@ struct ScanArgs {
   int L, D, N, softplus, vec_rows, vec_bc, chunks;
 };
 
+constexpr int kScanThreads = 128, kScanAhead = 32;
+
+template <int NPT, int LPC>
+struct ScanShape {
+  static constexpr int NP = NPT * LPC;              // padded states per channel
+  static constexpr int CT = kScanThreads / LPC;     // channels per block
+  static constexpr int TT = 64;                     // tokens per tile of B and C
+  static constexpr int G = 2 * LPC;                 // tokens per double group
+  static constexpr int PF = G >= kScanAhead ? 1 : kScanAhead / G;  // double groups ahead
+  static constexpr int BV = NP >= 8 ? 8 : NP;       // states per access of B and C
+  static constexpr int BITEMS = TT * (NP / BV);
+  static constexpr int BIPT = (BITEMS + kScanThreads - 1) / kScanThreads;
+  static constexpr int SMEM = 2 * TT * NP * 4;
+  static constexpr int BLOCKS = NP > 16 ? 2 : 4;    // per SM that the registers allow: 16 states, 4 sequences: 506 us, with 2 blocks 631
+};
+
 template <class T, int NPT, int LPC>
-__global__ void __launch_bounds__(kScanThreads) k_ssm_scan(const __grid_constant__ ScanArgs<T> a) {
+__global__ void __launch_bounds__(kScanThreads, ScanShape<NPT, LPC>::BLOCKS) k_ssm_scan(const __grid_constant__ ScanArgs<T> a) {
   using S = ScanShape<NPT, LPC>;
-  constexpr int NP = S::NP, CT = S::CT, TT = S::TT, V = S::V, BV = S::BV, BIPT = S::BIPT;
-  static_assert(S::ITEMS <= kScanThreads && TT % LPC == 0, "one row access per thread and tile");
+  constexpr int NP = S::NP, CT = S::CT, TT = S::TT, BV = S::BV, BIPT = S::BIPT, PF = S::PF, G = S::G;
+  constexpr int H = NPT / 2;  // pairs of states, for packed arithmetic
+  static_assert(TT % (PF * G) == 0, "whole rounds of groups per tile");
   extern __shared__ __align__(16) float smem[];
-  float2 *su = reinterpret_cast<float2 *>(smem);  // [TT][CT] {dt, dt * x}
-  float *sb = smem + 2 * TT * CT;                 // [TT][NP]
-  float *sc = sb + TT * NP;
-  float *sy = sc + TT * NP;                       // [TT][CT]
+  float *sb = smem, *sc = smem + TT * NP;
   pdl_trigger();
   pdl_wait();
   const int tid = threadIdx.x;
   const int64_t b = blockIdx.x / a.chunks;
-  const int c0 = (int)(blockIdx.x % a.chunks) * CT;
+  const int c = (int)(blockIdx.x % a.chunks) * CT + tid / LPC;
+  const int q = tid % LPC, n0 = q * NPT;
   const int T_b = seq_len(a.lengths, b, a.L);
-  const int tiles = (T_b + TT - 1) / TT;
+  const bool live = c < a.D;
 
-  // the states of this thread
-  const int ch = tid / LPC, q = tid % LPC, n0 = q * NPT;
-  const bool live = c0 + ch < a.D;
   float A2[NPT], h[NPT];
 #pragma unroll
   for (int i = 0; i < NPT; ++i) {
-    const int64_t at = (int64_t)(c0 + ch) * a.N + n0 + i;
+    const int64_t at = (int64_t)c * a.N + n0 + i;
     const bool on = live && n0 + i < a.N;
     A2[i] = on ? a.A[at] * kLog2e : 0.f;
     h[i] = on && a.state ? a.state[b * (int64_t)a.D * a.N + at] : 0.f;
   }
+  const float bias = live && a.dt_bias ? a.dt_bias[c] : 0.f, skip = live && a.skip ? a.skip[c] : 0.f;
 
-  // the row access of this thread: token rt of a tile, channels c0 + rc ...
-  const bool loads = tid < S::ITEMS;
-  const int rt = tid / (CT / V), rc = tid % (CT / V) * V;
-  const int have = loads ? min(V, a.D - c0 - rc) : 0;  // may be <= 0 behind the last channel
-  float bias[V], skip[V];
+  // this lane's rows: tokens q, q + LPC, ...
+  const T *px = a.x.at(b, q, c), *pd = a.dt.at(b, q, c), *pz = a.z.p ? a.z.at(b, q, c) : px;
+  T *po = a.out.at(b, q, c);
+  const int64_t sx = LPC * a.x.ldl, sd = LPC * a.dt.ldl, sz = LPC * (a.z.p ? a.z.ldl : a.x.ldl), so = LPC * a.out.ldl;
+  const int mine = live ? T_b - q : 0;  // a group that starts at t holds a token of this lane if t < mine
+  T nx[PF][2], nd[PF][2], nz[PF][2];
+  auto fetch = [&](int k, int t) {
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
-    bias[e] = e < have && a.dt_bias ? a.dt_bias[c0 + rc + e] : 0.f;
-    skip[e] = e < have && a.skip ? a.skip[c0 + rc + e] : 0.f;
-  }
-  Pack<T, V> nx, nd, nz;
-  Pack<T, BV> nb[BIPT], nc[BIPT];
-  auto fetch = [&](int tile) {
-    const int t = tile * TT + rt;
-    const int h_ = t < T_b ? have : 0;
-    nx.load(a.x.at(b, t, c0 + rc), a.vec_rows, h_);
-    nd.load(a.dt.at(b, t, c0 + rc), a.vec_rows, h_);
-    if (a.z.p) nz.load(a.z.at(b, t, c0 + rc), a.vec_rows, h_);
-#pragma unroll
-    for (int i = 0; i < BIPT; ++i) {
-      const int it = tid + i * kScanThreads, bt = it / (NP / BV), bn = it % (NP / BV) * BV;
-      const int t2 = tile * TT + bt;
-      const int hb = it < S::BITEMS && t2 < T_b ? a.N - bn : 0;
-      nb[i].load(a.bm.at(b, t2, bn), a.vec_bc, hb);
-      nc[i].load(a.cm.at(b, t2, bn), a.vec_bc, hb);
+    for (int w = 0; w < 2; ++w) {
+      const bool on = t + w * LPC < mine;
+      nx[k][w] = on ? *px : from_f<T>(0.f);
+      nd[k][w] = on ? *pd : from_f<T>(0.f);
+      nz[k][w] = on ? *pz : from_f<T>(0.f);
+      px += sx, pd += sd, pz += sz;
     }
   };
-  fetch(0);
-  for (int tile = 0; tile < tiles; ++tile) {
-    const Pack<T, V> x = nx, z = nz;
-    const bool tok = tile * TT + rt < T_b;
-    if (loads) {
+  Pack<T, BV> nb[BIPT], nc[BIPT];
+  auto fetch_bc = [&](int t0) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        float d = to_f(nd.v[e]) + bias[e];
-        if (a.softplus) d = softplus(d);
-        if (!tok) d = 0.f;  // behind the end: a = 1, no input
-        su[rt * CT + rc + e] = make_float2(d, d * to_f(x.v[e]));
-      }
+    for (int i = 0; i < BIPT; ++i) {
+      const int it = tid + i * kScanThreads, t = t0 + it / (NP / BV), n = it % (NP / BV) * BV;
+      const int have = it < S::BITEMS && t < T_b ? a.N - n : 0;
+      nb[i].load(a.bm.at(b, t, n), a.vec_bc, have);
+      nc[i].load(a.cm.at(b, t, n), a.vec_bc, have);
     }
+  };
+#pragma unroll
+  for (int k = 0; k < PF; ++k) fetch(k, k * G);
+  fetch_bc(0);
+  for (int t0 = 0; t0 < T_b; t0 += TT) {
+    if (t0) __syncthreads();  // the tile before has been read
 #pragma unroll
     for (int i = 0; i < BIPT; ++i) {
       const int it = tid + i * kScanThreads, at = it / (NP / BV) * NP + it % (NP / BV) * BV;
@@ -369,55 +378,314 @@ __global__ void __launch_bounds__(kScanThreads) k_ssm_scan(const __grid_constant
       }
     }
     __syncthreads();
-    if (tile + 1 < tiles) fetch(tile + 1);
+    fetch_bc(t0 + TT);
 #pragma unroll 1
-    for (int t = 0; t < TT; t += LPC) {
-      float p[LPC];
+    for (int g = 0; g < TT && t0 + g < T_b; g += PF * G) {
 #pragma unroll
-      for (int j = 0; j < LPC; ++j) {
-        const float2 u = su[(t + j) * CT + ch];
-        const float *bp = sb + (t + j) * NP + n0, *cp = sc + (t + j) * NP + n0;
-        float acc = 0.f;
+      for (int k = 0; k < PF; ++k) {
+        const int t = t0 + g + k * G;
+        const float2 x = make_float2(to_f(nx[k][0]), to_f(nx[k][1])), z = make_float2(to_f(nz[k][0]), to_f(nz[k][1]));
+        float2 d = __fadd2_rn(make_float2(to_f(nd[k][0]), to_f(nd[k][1])), make_float2(bias, bias));
+        fetch(k, t + PF * G);
+        if (a.softplus) d = softplus2(d);
+        const bool on0 = t < mine, on1 = t + LPC < mine;
+        d = make_float2(on0 ? d.x : 0.f, on1 ? d.y : 0.f);  // behind the end: a = 1, no input
+        const float2 u = __fmul2_rn(d, x);
+        float ys[2];
 #pragma unroll
-        for (int i = 0; i < NPT; ++i) {
-          h[i] = fmaf(ex2_approx(u.x * A2[i]), h[i], u.y * bp[i]);
-          acc = fmaf(cp[i], h[i], acc);
+        for (int w = 0; w < 2; ++w) {
+          float p[LPC];
+#pragma unroll
+          for (int j = 0; j < LPC; ++j) {
+            const float dj = __shfl_sync(0xffffffffu, w ? d.y : d.x, j, LPC);
+            const float uj = __shfl_sync(0xffffffffu, w ? u.y : u.x, j, LPC);
+            const float *bp = sb + (g + k * G + w * LPC + j) * NP + n0, *cp = sc + (g + k * G + w * LPC + j) * NP + n0;
+            if constexpr (NPT == 1) {
+              h[0] = fmaf(ex2_approx(dj * A2[0]), h[0], uj * bp[0]);
+              p[j] = cp[0] * h[0];
+            } else {
+              const float2 d2 = make_float2(dj, dj), u2 = make_float2(uj, uj);
+              Pack<float, NPT> Bv, Cv;
+              Bv.load_all(bp);
+              Cv.load_all(cp);
+              float2 acc = make_float2(0.f, 0.f);
+#pragma unroll
+              for (int i = 0; i < H; ++i) {
+                const float2 e = __fmul2_rn(d2, make_float2(A2[2 * i], A2[2 * i + 1]));
+                float2 hv = make_float2(h[2 * i], h[2 * i + 1]);
+                hv = __ffma2_rn(make_float2(ex2_approx(e.x), ex2_approx(e.y)), hv,
+                                __fmul2_rn(u2, make_float2(Bv.v[2 * i], Bv.v[2 * i + 1])));
+                h[2 * i] = hv.x, h[2 * i + 1] = hv.y;
+                const float2 C2 = make_float2(Cv.v[2 * i], Cv.v[2 * i + 1]);
+                acc = i ? __ffma2_rn(C2, hv, acc) : __fmul2_rn(C2, hv);
+              }
+              p[j] = acc.x + acc.y;
+            }
+          }
+#pragma unroll
+          for (int o = LPC / 2; o; o >>= 1) {
+            const bool up = q & o;
+#pragma unroll
+            for (int j = 0; j < o; ++j) {
+              const float keep = up ? p[j + o] : p[j], give = up ? p[j] : p[j + o];
+              p[j] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+            }
+          }
+          ys[w] = p[0];
         }
-        p[j] = acc;
+        float2 y = __ffma2_rn(make_float2(skip, skip), x, make_float2(ys[0], ys[1]));
+        if (a.z.p) y = __fmul2_rn(y, silu2(z));
+        if (on0) *po = from_f<T>(y.x);
+        po += so;
+        if (on1) *po = from_f<T>(y.y);
+        po += so;
       }
-#pragma unroll
-      for (int o = LPC / 2; o; o >>= 1) {
-        const bool up = q & o;
-#pragma unroll
-        for (int j = 0; j < o; ++j) {
-          const float keep = up ? p[j + o] : p[j], give = up ? p[j] : p[j + o];
-          p[j] = keep + __shfl_xor_sync(0xffffffffu, give, o);
-        }
-      }
-      sy[(t + q) * CT + ch] = p[0];  // lane q holds token t + q
-    }
-    __syncthreads();
-    if (loads && tok) {
-      Pack<T, V> o;
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        float y = fmaf(skip[e], to_f(x.v[e]), sy[rt * CT + rc + e]);
-        if (a.z.p) y *= silu(to_f(z.v[e]));
-        o.v[e] = from_f<T>(y);
-      }
-      o.store(a.out.at(b, tile * TT + rt, c0 + rc), a.vec_rows, have);
     }
   }
-  // outputs behind the end are zeros
-  if (loads) {
-    Pack<T, V> o;
-    o.zero();
-    for (int t = T_b + rt; t < a.L; t += TT) o.store(a.out.at(b, t, c0 + rc), a.vec_rows, have);
+  if (live) {  // outputs behind the end are zeros
+    for (int t = T_b + q; t < a.L; t += LPC) *a.out.at(b, t, c) = from_f<T>(0.f);
   }
   if (a.state && live && T_b > 0) {
 #pragma unroll
     for (int i = 0; i < NPT; ++i)
-      if (n0 + i < a.N) a.state[(b * a.D + c0 + ch) * (int64_t)a.N + n0 + i] = h[i];
+      if (n0 + i < a.N) a.state[(b * a.D + c) * (int64_t)a.N + n0 + i] = h[i];
+  }
+}
+
+// ------------------------------------------------------------ selective scan, prompts: lanes share the tokens
+// For sequences with few channels, whose tokens one after the other would leave most of the
+// schedulers without a warp.  A lane owns two channels (packed arithmetic) and kTimeItems
+// consecutive tokens, 32 lanes a tile of 32 * kTimeItems tokens.  For each state the lane first runs
+// its tokens from zero, the lanes join their (decay, end state) pairs in five shuffle rounds,
+// then the lane runs its tokens again from the state that reaches it: the exponentials are
+// taken once and kept for both runs.  Two states at a time, for two independent chains.  B and C
+// are staged in fp32 for chunks of 16 states (any N), x, dt and z as planes of channel pairs; the
+// next tile's rows are loaded while one is computed.
+// One bf16 sequence of 8192 tokens, 2048 channels, 16 states: 226 us, against 532 us of the kernel
+// above; at 8192 channels 394 us against 340.  It issues 12 instructions per state at 0.4 of
+// the rate: 7 warps per SM, held back by the shuffle rounds (a fifth of the time).
+constexpr int kTimeItems = 8, kTimeStates = 16, kTimePairs = 4;  // tokens per lane; states per chunk; warps per block
+
+template <class T>
+struct TimeShape {
+  static constexpr int I = kTimeItems, TT = 32 * I, CH = 2 * kTimePairs, THREADS = 32 * kTimePairs;
+  // planes of one channel pair, [I][ROW]: rows 4 words apart modulo 32, for the staging stores (lanes along I)
+  static constexpr int ROW = 32 + 4, PITCH = I * ROW;
+  // planes of one state, [I / 2][BROW] of two items' values
+  static constexpr int BROW = 2 * 32 + 8, BPLANE = I / 2 * BROW, BC = kTimeStates * BPLANE;
+  static constexpr int XIT = TT / THREADS, BIT = TT * (kTimeStates / 8) / THREADS;  // accesses per thread and tile
+  static int smem(int N) { return 4 * (2 * BC + 4 * ((N + 1) & ~1) * kTimePairs) + 3 * 2 * (int)sizeof(T) * kTimePairs * PITCH; }
+};
+
+template <class T>
+struct alignas(2 * sizeof(T)) Pair {
+  T a, b;
+  __device__ __forceinline__ float2 f() const { return make_float2(to_f(a), to_f(b)); }
+};
+
+template <class T>
+__global__ void __launch_bounds__(TimeShape<T>::THREADS, 1) k_ssm_scan_time(const __grid_constant__ ScanArgs<T> a) {
+  using S = TimeShape<T>;
+  constexpr int I = S::I, TT = S::TT, CH = S::CH, ROW = S::ROW, PITCH = S::PITCH, BROW = S::BROW, BPLANE = S::BPLANE;
+  constexpr int THREADS = S::THREADS, XIT = S::XIT, BIT = S::BIT, NC = kTimeStates, PAIRS = kTimePairs;
+  static_assert(CH == 8 && TT % THREADS == 0, "one access of 8 channels per token");
+  extern __shared__ __align__(16) float smem[];
+  const int Np = (a.N + 1) & ~1;                                // states two at a time: zeros behind the last
+  float *sb = smem, *sc = sb + S::BC;                           // [NC][I / 2][BROW]
+  float2 *sa = reinterpret_cast<float2 *>(sc + S::BC);          // [Np][PAIRS] A log2(e)
+  float2 *sh = sa + Np * PAIRS;                                 // [Np][PAIRS] state at the tile's start
+  Pair<T> *sx = reinterpret_cast<Pair<T> *>(sh + Np * PAIRS);   // [PAIRS][I][ROW]
+  Pair<T> *sd = sx + PAIRS * PITCH, *sz = sd + PAIRS * PITCH;
+  pdl_trigger();
+  pdl_wait();
+  const int tid = threadIdx.x, tl = tid & 31, pair = tid >> 5;
+  const int64_t b = blockIdx.x / a.chunks;
+  const int c0 = (int)(blockIdx.x % a.chunks) * CH, c = c0 + 2 * pair;
+  const int T_b = seq_len(a.lengths, b, a.L);
+  const int live = min(2, a.D - c);  // channels of this warp's pair that exist
+  float *state = a.state ? a.state + (b * a.D + c) * (int64_t)a.N : nullptr;
+
+  for (int n = tl; n < Np; n += 32) {
+    float2 A = make_float2(0.f, 0.f), h = A;
+    const int64_t at = (int64_t)c * a.N + n;
+    if (n < a.N && live > 0) A.x = a.A[at] * kLog2e, h.x = state ? state[n] : 0.f;
+    if (n < a.N && live > 1) A.y = a.A[at + a.N] * kLog2e, h.y = state ? state[a.N + n] : 0.f;
+    sa[n * PAIRS + pair] = A;
+    sh[n * PAIRS + pair] = h;
+  }
+  const float2 bias = make_float2(a.dt_bias && live > 0 ? a.dt_bias[c] : 0.f, a.dt_bias && live > 1 ? a.dt_bias[c + 1] : 0.f);
+  const float2 skip = make_float2(a.skip && live > 0 ? a.skip[c] : 0.f, a.skip && live > 1 ? a.skip[c + 1] : 0.f);
+
+  Pack<T, CH> px[XIT], pd[XIT], pz[XIT];
+  Pack<T, 8> pb[BIT], pc[BIT];
+  auto fetch_rows = [&](int t0) {
+#pragma unroll
+    for (int k = 0; k < XIT; ++k) {
+      const int t = t0 + tid + k * THREADS, have = t < T_b ? a.D - c0 : 0;
+      px[k].load(a.x.at(b, t, c0), a.vec_rows, have);
+      pd[k].load(a.dt.at(b, t, c0), a.vec_rows, have);
+      if (a.z.p) pz[k].load(a.z.at(b, t, c0), a.vec_rows, have);
+    }
+  };
+  auto fetch_bc = [&](int t0, int n0) {
+#pragma unroll
+    for (int k = 0; k < BIT; ++k) {
+      const int it = tid + k * THREADS, t = t0 + it % TT, n = n0 + it / TT * 8;
+      const int have = t < T_b ? a.N - n : 0;
+      pb[k].load(a.bm.at(b, t, n), a.vec_bc, have);
+      pc[k].load(a.cm.at(b, t, n), a.vec_bc, have);
+    }
+  };
+  fetch_rows(0);
+  fetch_bc(0, 0);
+  for (int t0 = 0; t0 < T_b; t0 += TT) {
+    __syncthreads();  // the rows of the tile before have been stored
+    // rows -> planes; token t of the tile is item t % I of lane t / I
+#pragma unroll
+    for (int k = 0; k < XIT; ++k) {
+      const int r = tid + k * THREADS, at = r % I * ROW + r / I;
+#pragma unroll
+      for (int e = 0; e < PAIRS; ++e) {
+        sx[at + e * PITCH] = Pair<T>{px[k].v[2 * e], px[k].v[2 * e + 1]};
+        sd[at + e * PITCH] = Pair<T>{pd[k].v[2 * e], pd[k].v[2 * e + 1]};
+        if (a.z.p) sz[at + e * PITCH] = Pair<T>{pz[k].v[2 * e], pz[k].v[2 * e + 1]};
+      }
+    }
+    float2 dt[I], u[I], y[I];
+    for (int n0 = 0; n0 < a.N; n0 += NC) {
+      if (n0) __syncthreads();  // the chunk before has been read
+#pragma unroll
+      for (int k = 0; k < BIT; ++k) {
+        const int it = tid + k * THREADS, r = it % TT, n = it / TT * 8, i = r % I, l = r / I;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int at = (n + e) * BPLANE + i / 2 * BROW + l * 2 + i % 2;
+          sb[at] = to_f(pb[k].v[e]);
+          sc[at] = to_f(pc[k].v[e]);
+        }
+      }
+      __syncthreads();
+      if (n0 + NC < a.N) fetch_bc(t0, n0 + NC);
+      else fetch_bc(t0 + TT, 0);
+      if (n0 == 0) {
+        fetch_rows(t0 + TT);
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+          const int at = pair * PITCH + i * ROW + tl;
+          const float2 x = sx[at].f();
+          float2 d = __fadd2_rn(sd[at].f(), bias);
+          if (a.softplus) d = softplus2(d);
+          if (t0 + tl * I + i >= T_b) d = make_float2(0.f, 0.f);  // behind the end: a = 1, no input
+          dt[i] = d;
+          u[i] = __fmul2_rn(d, x);
+          y[i] = __fmul2_rn(skip, x);
+        }
+      }
+      const int nn = min(NC, Np - n0);
+      auto values = [&](const float *p, int n, int i) {  // of items i, i + 1
+        return reinterpret_cast<const float2 *>(p)[(n * BPLANE + i / 2 * BROW) / 2 + tl];
+      };
+#pragma unroll 1
+      for (int n = 0; n < nn; n += 2) {
+        float2 A[2], start[2], ea[2][I], in[2][I], h[2], P[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          A[k] = sa[(n0 + n + k) * PAIRS + pair];
+          start[k] = sh[(n0 + n + k) * PAIRS + pair];
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int i = 0; i < I; i += 2) {
+            const float2 B2 = values(sb, n + k, i);
+            in[k][i] = __fmul2_rn(u[i], make_float2(B2.x, B2.x));
+            in[k][i + 1] = __fmul2_rn(u[i + 1], make_float2(B2.y, B2.y));
+          }
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float2 e = __fmul2_rn(dt[i], A[k]);
+            ea[k][i] = make_float2(ex2_approx(e.x), ex2_approx(e.y));
+          }
+        // this lane's tokens from zero (the first lane: from the tile's state), and its decay
+#pragma unroll
+        for (int k = 0; k < 2; ++k) h[k] = in[k][0], P[k] = ea[k][0];
+        if (tl == 0) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) h[k] = __ffma2_rn(ea[k][0], start[k], h[k]);
+        }
+#pragma unroll
+        for (int i = 1; i < I; ++i)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            h[k] = __ffma2_rn(ea[k][i], h[k], in[k][i]);
+            P[k] = __fmul2_rn(P[k], ea[k][i]);
+          }
+        if (tl == 0) {  // nothing lies before it; lanes that reach it take over its 0, so that no round needs a test
+#pragma unroll
+          for (int k = 0; k < 2; ++k) P[k] = make_float2(0.f, 0.f);
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float2 hu = make_float2(__shfl_up_sync(0xffffffffu, h[k].x, o), __shfl_up_sync(0xffffffffu, h[k].y, o));
+            h[k] = __ffma2_rn(P[k], hu, h[k]);
+            if (o < 16)
+              P[k] = __fmul2_rn(P[k], make_float2(__shfl_up_sync(0xffffffffu, P[k].x, o), __shfl_up_sync(0xffffffffu, P[k].y, o)));
+          }
+        float2 g[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          g[k] = make_float2(__shfl_up_sync(0xffffffffu, h[k].x, 1), __shfl_up_sync(0xffffffffu, h[k].y, 1));
+          if (tl == 0) g[k] = start[k];
+        }
+#pragma unroll
+        for (int i = 0; i < I; i += 2)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float2 C2 = values(sc, n + k, i);
+            g[k] = __ffma2_rn(ea[k][i], g[k], in[k][i]);
+            y[i] = __ffma2_rn(make_float2(C2.x, C2.x), g[k], y[i]);
+            g[k] = __ffma2_rn(ea[k][i + 1], g[k], in[k][i + 1]);
+            y[i + 1] = __ffma2_rn(make_float2(C2.y, C2.y), g[k], y[i + 1]);
+          }
+        if (tl == 31) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) sh[(n0 + n + k) * PAIRS + pair] = h[k];
+        }
+      }
+    }
+    // gate, then back through the planes of x into rows
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      const int at = pair * PITCH + i * ROW + tl;
+      float2 o = y[i];
+      if (a.z.p) o = __fmul2_rn(o, silu2(sz[at].f()));
+      sx[at] = Pair<T>{from_f<T>(o.x), from_f<T>(o.y)};
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < XIT; ++k) {
+      const int r = tid + k * THREADS, at = r % I * ROW + r / I;
+      if (t0 + r >= T_b) continue;
+      Pack<T, CH> o;
+#pragma unroll
+      for (int e = 0; e < PAIRS; ++e) o.v[2 * e] = sx[at + e * PITCH].a, o.v[2 * e + 1] = sx[at + e * PITCH].b;
+      o.store(a.out.at(b, t0 + r, c0), a.vec_rows, a.D - c0);
+    }
+  }
+  Pack<T, CH> zero;  // outputs behind the end
+  zero.zero();
+  for (int t = T_b + tid; t < a.L; t += THREADS) zero.store(a.out.at(b, t, c0), a.vec_rows, a.D - c0);
+  if (state && T_b > 0) {
+    __syncwarp();
+    for (int n = tl; n < a.N; n += 32) {
+      const float2 h = sh[n * PAIRS + pair];
+      if (live > 0) state[n] = h.x;
+      if (live > 1) state[a.N + n] = h.y;
+    }
   }
 }
 
@@ -563,28 +831,20 @@ __global__ void __launch_bounds__(kStepThreads, 5) k_ssm_step(const __grid_const
   }
 }
 
+template <class K, class A>
+static int launch_scan_k(K kern, const A &a, int64_t blocks, int threads, int smem, cudaStream_t st) {
+  if (smem > 48 * 1024) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return fail(TESM_ELAUNCH, std::string("ssm_scan: ") + cudaGetErrorString(e));
+  }
+  return launch_k("ssm_scan", kern, dim3((unsigned)blocks), dim3(threads), smem, st, a);
+}
+
 template <class T, int NPT, int LPC>
 static int launch_scan(ScanArgs<T> a, int64_t B, cudaStream_t st) {
   using S = ScanShape<NPT, LPC>;
-  if constexpr (S::SMEM > 48 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(k_ssm_scan<T, NPT, LPC>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
-    if (e != cudaSuccess) return fail(TESM_ELAUNCH, std::string("ssm_scan: ") + cudaGetErrorString(e));
-  }
   a.chunks = (int)ceil_div(a.D, S::CT);
-  return launch_k("ssm_scan", k_ssm_scan<T, NPT, LPC>, dim3((unsigned)(B * a.chunks)), dim3(kScanThreads), S::SMEM, st,
-                  a);
-}
-
-template <class T, int NPT>
-static int launch_scan_lanes(const ScanArgs<T> &a, int64_t B, int lpc, cudaStream_t st) {
-  switch (lpc) {
-    case 1: return launch_scan<T, NPT, 1>(a, B, st);
-    case 2: return launch_scan<T, NPT, 2>(a, B, st);
-    case 4: return launch_scan<T, NPT, 4>(a, B, st);
-    case 8: return launch_scan<T, NPT, 8>(a, B, st);
-    case 16: return launch_scan<T, NPT, 16>(a, B, st);
-    default: return launch_scan<T, NPT, 32>(a, B, st);
-  }
+  return launch_scan_k(k_ssm_scan<T, NPT, LPC>, a, B * a.chunks, kScanThreads, S::SMEM, st);
 }
 
 template <class T, int LPC>
@@ -610,14 +870,24 @@ static int ssm_scan_t(ScanArgs<T> a, int64_t B, cudaStream_t st) {
       default: return launch_step<T, 32>(a, B, st);
     }
   }
-  // States per lane: as many as still give every SM a block; fewer states per lane spread a
-  // channel over more lanes.
-  int npt = np >= 4 ? 4 : np;
-  while (npt > 1 && np / (npt / 2) <= 32 && B * ceil_div((int64_t)a.D * (np / npt), kScanThreads) < sm_count()) npt >>= 1;
-  const int lpc = np / npt;
-  return npt == 4   ? launch_scan_lanes<T, 4>(a, B, lpc, st)
-         : npt == 2 ? launch_scan_lanes<T, 2>(a, B, lpc, st)
-                    : launch_scan_lanes<T, 1>(a, B, lpc, st);
+  // Warps of the kernel whose lanes share the states: 4 states per lane.  With fewer than there are
+  // schedulers the lanes share the tokens instead, where the sequences fill half a tile of them and
+  // the rows can be staged by 16-byte accesses (unaligned fp32 rows, 578 warps: 42 us against 29).
+  const int64_t warps = ceil_div(B * a.D * (int64_t)np, 128);
+  if (warps < 4 * (int64_t)sm_count() && a.L >= TimeShape<T>::TT / 2 && a.vec_rows) {
+    a.chunks = (int)ceil_div(a.D, TimeShape<T>::CH);
+    return launch_scan_k(k_ssm_scan_time<T>, a, B * a.chunks, TimeShape<T>::THREADS, TimeShape<T>::smem(a.N), st);
+  }
+  switch (np) {
+    case 1: return launch_scan<T, 1, 1>(a, B, st);
+    case 2: return launch_scan<T, 2, 1>(a, B, st);
+    case 4: return launch_scan<T, 4, 1>(a, B, st);
+    case 8: return launch_scan<T, 4, 2>(a, B, st);
+    case 16: return launch_scan<T, 4, 4>(a, B, st);
+    case 32: return launch_scan<T, 4, 8>(a, B, st);
+    case 64: return launch_scan<T, 4, 16>(a, B, st);
+    default: return launch_scan<T, 4, 32>(a, B, st);
+  }
 }
 
 template <class T, int N, int U>

@@ -270,6 +270,53 @@ def test_scan_lane_splits(N, C):
 
 
 @DT
+@pytest.mark.parametrize("L", [127, 128, 255, 256, 257, 700])
+@pytest.mark.parametrize("C,N", [(8, 16), (4, 3), (40, 1), (16, 17), (24, 33), (8, 128)])
+def test_scan_few_channels(C, N, L, dtype):
+    """Few channels and many tokens, at which lanes share the tokens: tiles of 256, chunks of 16 states."""
+    check_scan(inputs(L + N, 2, L, C, N, dtype))
+
+
+@DT
+@pytest.mark.parametrize("gate,state,skip", [(False, True, False), (True, False, True), (False, False, False)])
+def test_scan_few_channels_ragged(gate, state, skip, dtype):
+    lengths = torch.tensor([0, 1, 300, 256, 8, 257], dtype=torch.int32)
+    kw = inputs(20, 6, 300, 24, 18, dtype, gate, state, skip)
+    for name in ("x", "dt", "Bm", "Cm", "z"):
+        for b, n in enumerate(lengths):
+            if name in kw:
+                kw[name][b, n:] = float("nan")
+    got = check_scan(kw, lengths=lengths)
+    assert torch.isfinite(got.float()).all()
+
+
+@DT
+def test_scan_few_channels_in_pieces_and_strided(dtype):
+    """The kernels for prompts and tokens continue one another; rows inside wider buffers."""
+    B, L, C, N = 2, 600, 16, 16
+    kw = inputs(21, B, L, C, N, dtype)
+    out, tol, h, eh = scan64(**kw)
+    a = cuda(kw)
+    proj = torch.full((B, L, 3 * C + 2 * N + 16), float("nan"), dtype=dtype, device="cuda")
+    at = 8
+    for name, n in (("x", C), ("dt", C), ("z", C), ("Bm", N), ("Cm", N)):
+        proj[..., at:at + n] = a[name]
+        a[name] = proj[..., at:at + n]
+        at += n
+    buf = torch.full((B, L, C + 16), 7.0, dtype=dtype, device="cuda")
+    for cuts in ([600], [300, 1, 128, 171], [40, 560]):
+        st, at = a["state"].clone(), 0
+        for n in cuts:
+            s = slice(at, at + n)
+            ops.ssm_scan(a["x"][:, s], a["dt"][:, s], a["A"], a["Bm"][:, s], a["Cm"][:, s], D=a["D"], z=a["z"][:, s],
+                         dt_bias=a["dt_bias"], state=st, out=buf[:, s, 8:8 + C])
+            at += n
+        assert ((buf[..., 8:8 + C].cpu().double() - out).abs() <= tol).all()
+        assert ((st.cpu().double() - h).abs() <= eh).all()
+        assert (buf[..., :8] == 7).all() and (buf[..., 8 + C:] == 7).all()
+
+
+@DT
 @pytest.mark.parametrize("gate,state,skip,bias,softplus", [(False, True, True, True, True), (True, False, False, False, True),
                                                            (False, False, False, False, False),
                                                            (True, True, True, True, False)])
