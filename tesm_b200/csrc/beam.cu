@@ -570,6 +570,9 @@ extern "C" int tesm_b200_reorder_states(const tesm_b200_state_rows *states, int6
     TESM_REQUIRE(s.src_stride >= s.row_bytes && s.dst_stride >= s.row_bytes, "reorder_states: rows overlap");
     TESM_REQUIRE(s.src != s.dst || (Win == Wout && s.src_stride == s.dst_stride),
                  "reorder_states: in place needs as many beams out as in");
+    const char *lo = (const char *)s.dst, *hi = lo + (G * Wout - 1) * s.dst_stride + s.row_bytes;
+    TESM_REQUIRE((const char *)(parents + G * Wout) <= lo || (const char *)parents >= hi,
+                 "reorder_states: parents lie inside a state");
   }
   StateTable t;
   t.n = 0;

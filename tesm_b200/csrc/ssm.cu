@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(kConvThreads)
   const int c = (chunk * kConvThreads + threadIdx.x) * N;
   if (c >= D) return;
   const int have = min(N, D - c);
-  constexpr bool kAsync = N * sizeof(T) == 16 && U > 1;
+  constexpr bool kAsync = N * sizeof(T) == 16 && U == 2;  // with D a multiple of N: whole accesses only
   constexpr int kGroups = 8;  // groups of U rows in shared memory
   __shared__ __align__(16) char smem[kAsync ? kGroups * U * kConvThreads * 16 : 16];
   const uint32_t slot = (uint32_t)__cvta_generic_to_shared(smem) + threadIdx.x * 16;
@@ -205,9 +205,8 @@ __global__ void __launch_bounds__(kConvThreads)
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           if constexpr (kAsync) {
-            if (t + u < te)
-              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot + (uint32_t)(t + u - t0) % (kGroups * U) * (kConvThreads * 16)),
-                           "l"(xp) : "memory");
+            const uint32_t at = (uint32_t)(t + u - t0) % (kGroups * U) * (kConvThreads * 16);
+            if (t + u < te) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot + at), "l"(xp) : "memory");
           } else {
             next[u].load(xp, vec, t + u < te ? have : 0);
           }
@@ -926,8 +925,10 @@ static int causal_conv_t(const void *x, int64_t ldb, int64_t ldl, int64_t B, int
   const uint64_t bits = (uintptr_t)x | (uintptr_t)y | (uintptr_t)state |
                         (uint64_t)((ldb | ldl | ldyb | ldyl | (state ? D : 0)) * (int64_t)sizeof(T));
   constexpr int N = 16 / sizeof(T);
-  if (bits % 16 == 0 && L >= 4)
+  if (bits % 16 == 0 && L >= 4 && D % N == 0)
     return launch_conv<T, N, 2>(rx, B, (int)L, (int)D, (int)K, 1, w, bias, (T *)state, lengths, act, ry, st);
+  if (bits % 16 == 0 && L >= 4)
+    return launch_conv<T, N, 4>(rx, B, (int)L, (int)D, (int)K, 1, w, bias, (T *)state, lengths, act, ry, st);
   if (bits % 16 == 0)
     return launch_conv<T, N, 1>(rx, B, (int)L, (int)D, (int)K, 1, w, bias, (T *)state, lengths, act, ry, st);
   return launch_conv<T, 1, 4>(rx, B, (int)L, (int)D, (int)K, 0, w, bias, (T *)state, lengths, act, ry, st);

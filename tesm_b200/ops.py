@@ -602,11 +602,13 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: Optional[int]
 
 def _row_layout(what: str, t: torch.Tensor, rows: int):
     """(data pointer, row bytes, row stride in bytes) of a tensor whose rows are dense."""
-    _need(t.dim() >= 1 and t.shape[0] == rows, f"{what}: a state of shape {tuple(t.shape)} has not {rows} rows")
+    if t.dim() < 1 or t.shape[0] != rows:
+        raise ValueError(f"tesm_b200 {what}: a state of shape {tuple(t.shape)} has not {rows} rows")
     n = 1
     for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
-        _need(size == 1 or stride == n, f"{what}: the rows of a state must be dense (shape {tuple(t.shape)}, strides "
-                                        f"{t.stride()})")
+        if size != 1 and stride != n:
+            raise ValueError(f"tesm_b200 {what}: the rows of a state must be dense (shape {tuple(t.shape)}, strides "
+                             f"{t.stride()})")
         n *= size
     es = t.element_size()
     stride = t.stride(0) if rows > 1 else n
@@ -632,7 +634,8 @@ class StateReorder:
     tensors; each column of rows is read into registers before it is stored, so no copy is kept.
     With ``out`` (tensors of prompts * beams rows) the rows come from ``states`` of prompts * ``beams_in``
     rows instead: beams_in = 1 and parents of zeros spreads one row per prompt over its beams.
-    A parent out of range leaves its row as it is and sets :func:`device_status` to 1."""
+    A parent out of range leaves its row as it is and sets :func:`device_status` to 1.  The plan holds
+    the tensors and their addresses: they stay where they are for its life."""
 
     def __init__(self, states: Sequence[torch.Tensor], beams: int, out: Optional[Sequence[torch.Tensor]] = None,
                  beams_in: Optional[int] = None):
@@ -654,13 +657,17 @@ class StateReorder:
         self._table = (_lib.StateRows * len(states))()
         src_rows, dst_rows = [], []
         for e, s, d in zip(self._table, states, dst):
-            _need(s.dtype == d.dtype and s.shape[1:] == d.shape[1:], f"{what}: a state and its output differ in type or "
-                                                                     f"row shape")
-            _no_grad(what, s, d)
             e.src, e.row_bytes, e.src_stride = _row_layout(what, s, rows_in)
-            e.dst, _, e.dst_stride = _row_layout(what, d, rows_out)
-            src_rows.append((s.data_ptr(), e.row_bytes, e.src_stride, rows_in))
-            dst_rows.append((d.data_ptr(), e.row_bytes, e.dst_stride, rows_out))
+            src_rows.append((e.src or 0, e.row_bytes, e.src_stride, rows_in))
+            if d is s:
+                e.dst, e.dst_stride = e.src, e.src_stride
+                dst_rows.append(src_rows[-1])
+            else:
+                _need(s.dtype == d.dtype and s.shape[1:] == d.shape[1:], f"{what}: a state and its output differ in type "
+                                                                         f"or row shape")
+                e.dst, _, e.dst_stride = _row_layout(what, d, rows_out)
+                dst_rows.append((e.dst or 0, e.row_bytes, e.dst_stride, rows_out))
+        _no_grad(what, *states, *dst)
         # what is written is written once, and nothing that another entry reads; sorted by address, a
         # set of rows can only meet those that begin before its end
         every = sorted([(r, True) for r in dst_rows] + ([(r, False) for r in src_rows] if out is not None else []))

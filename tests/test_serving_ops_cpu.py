@@ -6,7 +6,7 @@ import torch
 
 from tesm_b200 import _lib, ops
 
-P = ctypes.c_void_p(4096)  # never dereferenced: the checks come first
+P = ctypes.c_void_p(1 << 20)  # never dereferenced: the checks come first
 
 
 def status(name, *args):
@@ -22,7 +22,7 @@ def beam(dtype=0, G=1, W=4, V=100, K=4, logits=P, scores=P, lengths=None, alpha=
                                      (dict(V=0), 1), (dict(V=1 << 31), 1), (dict(G=-1), 1), (dict(G=1 << 23), 1),
                                      (dict(logits=None), 1), (dict(scores=None), 1), (dict(alpha=1.0), 1),
                                      (dict(alpha=float("nan"), lengths=P), 1), (dict(pad=-1), 1), (dict(ws=None), 1),
-                                     (dict(ws_bytes=15), 1), (dict(ws=ctypes.c_void_p(4104)), 1), (dict(G=0), 0)])
+                                     (dict(ws_bytes=15), 1), (dict(ws=ctypes.c_void_p((1 << 20) + 8)), 1), (dict(G=0), 0)])
 def test_beam_select_refuses(kw, want):
     assert beam(**kw) == want
     if want:
@@ -51,11 +51,18 @@ def rows(*entries):
     ((4096, None, 64, 64, 64), 2, 4, 4, P, 1), ((4096, 4096, 64, 32, 64), 2, 4, 4, P, 1),
     ((4096, 4096, 64, 64, 32), 2, 4, 4, P, 1), ((4096, 4096, -1, 64, 64), 2, 4, 4, P, 1),
     ((4096, 4096, 64, 64, 64), 2, 1, 4, P, 1), ((4096, 4096, 64, 64, 128), 2, 4, 4, P, 1),
-    ((4096, 4096, 1 << 36, 1 << 36, 1 << 36), 2, 4, 4, P, 5), ((4096, 4096, 64, 64, 64), 0, 4, 4, P, 0),
+    ((4096, 4096, 1 << 36, 1 << 36, 1 << 36), 2, 4, 4, ctypes.c_void_p(1 << 60), 5), ((4096, 4096, 64, 64, 64), 0, 4, 4, P, 0),
     ((4096, 4096, 0, 0, 0), 2, 4, 4, P, 0)])
 def test_reorder_refuses(entry, G, Win, Wout, parents, want):
     t = rows(entry)
     assert status("tesm_b200_reorder_states", ctypes.addressof(t), 1, G, Win, Wout, parents, None) == want
+
+
+@pytest.mark.parametrize("parents", [4096, 4096 + 60, 4096 + 7 * 64 + 63, 4096 - 4])
+def test_reorder_refuses_parents_inside_a_state(parents):
+    t = rows((4096, 4096, 64, 64, 64))
+    assert status("tesm_b200_reorder_states", ctypes.addressof(t), 1, 2, 4, 4, ctypes.c_void_p(parents), None) == 1
+    assert "parents" in _lib.last_error()
 
 
 def test_reorder_refuses_no_table():
@@ -63,7 +70,7 @@ def test_reorder_refuses_no_table():
     assert status("tesm_b200_reorder_states", None, 0, 2, 4, 4, P, None) == 0
 
 
-def conv(dtype=0, B=1, L=4, D=8, K=4, x=P, w=P, out=P):
+def conv(dtype=0, B=1, L=4, D=8, K=4, x=P, w=P, out=P):  # checks that come before the ones on shared memory
     return status("tesm_b200_causal_conv", x, dtype, 32, 8, B, L, D, K, w, None, None, None, 1, out, 32, 8, None)
 
 

@@ -105,24 +105,27 @@ def test_conv_lengths_and_garbage_behind_them(dtype):
 
 
 @DT
+@pytest.mark.parametrize("D", [48, 20, 6])
 @pytest.mark.parametrize("off", [0, 1, 4, 8])
-def test_conv_strided_rows(off, dtype):
-    """x and out as slices of wider buffers, at every alignment, batch innermost of the two."""
-    B, L, D = 3, 37, 48
+def test_conv_strided_rows(off, D, dtype):
+    """x and out as slices of wider buffers, at every alignment, batch innermost of the two; channels
+    that end inside a 16-byte access."""
+    B, L = 3, 37
+    pad = 16 + -D % 8
 
     def wide(x):
-        buf = torch.full((L, B, D + 16), float("nan"), dtype=dtype, device="cuda")
+        buf = torch.full((L, B, D + pad), float("nan"), dtype=dtype, device="cuda")
         v = buf[:, :, off:off + D].transpose(0, 1)
         v.copy_(x)
         return v
 
     x, w, s = rand(1, B, L, D, dtype=dtype), rand(2, D, 4), rand(3, B, 3, D, dtype=dtype)
     a = check_conv(x, w, None, s, view=wide)
-    buf = torch.full((B, L, D + 16), 7.0, dtype=dtype, device="cuda")
+    buf = torch.full((B, L, D + pad), 7.0, dtype=dtype, device="cuda")
     st = s.cuda()
     r = ops.causal_conv(x.cuda(), w.cuda(), state=st, out=buf[:, :, off:off + D])
     assert r.data_ptr() == buf[:, :, off:off + D].data_ptr() and torch.equal(r, a)
-    rest = torch.ones(D + 16, dtype=torch.bool)
+    rest = torch.ones(D + pad, dtype=torch.bool)
     rest[off:off + D] = False
     assert (buf[:, :, rest.cuda()] == 7).all()
 
@@ -357,9 +360,10 @@ def test_scan_extreme_steps():
 
 @DT
 @pytest.mark.parametrize("off", [0, 1, 4, 8])
-def test_scan_strided_inputs(off, dtype):
+@pytest.mark.parametrize("L,C,N", [(45, 24, 8), (1, 24, 8), (260, 24, 8), (1, 20, 6)])
+def test_scan_strided_inputs(L, C, N, off, dtype):
     """All inputs as slices of one projection, at every alignment; out inside a wider buffer."""
-    B, L, C, N = 2, 45, 24, 8
+    B = 2
     kw = inputs(9, B, L, C, N, dtype)
     a = cuda(kw)
     want_state = a["state"].clone()
@@ -375,7 +379,11 @@ def test_scan_strided_inputs(off, dtype):
     out = buf[..., off:off + C]
     got = ops.ssm_scan(a["x"], a["dt"], a["A"], a["Bm"], a["Cm"], D=a["D"], z=a["z"], dt_bias=a["dt_bias"],
                        state=a["state"], out=out)
-    assert got is out and torch.equal(got, want) and torch.equal(a["state"], want_state)
+    assert got is out
+    if L < 128:  # the same kernel
+        assert torch.equal(got, want) and torch.equal(a["state"], want_state)
+    ref, tol, h, eh = scan64(**kw)
+    assert ((got.cpu().double() - ref).abs() <= tol).all() and ((a["state"].cpu().double() - h).abs() <= eh).all()
     rest = torch.ones(C + 16, dtype=torch.bool)
     rest[off:off + C] = False
     assert (buf[:, :, rest.cuda()] == 7).all()
