@@ -278,12 +278,12 @@ __global__ void __launch_bounds__(kConvThreads)
 // partial sums exchange halves in log2(LPC) rounds), which gates and stores it.  So the
 // per-channel work is done once, and only B and C, shared by all channels, go through shared
 // memory, in fp32 tiles of 64 tokens.
-// Bytes do not bound it (41 us for one bf16 prompt of 4096 tokens, 8192 channels, 16 states), nor
-// the 20 exponentials and reciprocals per token and channel (149 us at 16 a clock and SM), but the 11
-// instructions per state at the issue rate of the 7 warps an SM gets from one sequence: 340 us; four
-// sequences of 2048 tokens, twice the work, take 506 us.
-// Inputs staged through shared memory with softplus formed by the loading thread took 354 us; 16 instead of
-// 32 tokens ahead 368 us; two states per lane (twice the warps, 16 instructions per state) 541 us.
+// One bf16 sequence of 4096 tokens, 8192 channels, 16 states: 340 us.  Neither its bytes bound it
+// (41 us) nor its 20 exponentials and reciprocals per token and channel (149 us at 16 a clock and
+// SM), but the 9 instructions per state, at 0.4 of the issue rate with the 7 warps that an SM
+// gets from one sequence; four sequences of 2048 tokens, twice the work, take 506 us.  Inputs staged
+// through shared memory with softplus formed by the loading thread took 354 us; 16 instead of 32
+// tokens ahead 368 us; two states per lane (twice the warps, narrower row accesses) 541 us.
 template <class T>
 struct ScanArgs {
   Rows<const T> x, dt, bm, cm, z;
@@ -695,7 +695,9 @@ __global__ void __launch_bounds__(TimeShape<T>::THREADS, 1) k_ssm_scan_time(cons
 // get them by shuffles, and the sums over the states end in that lane again (transposed
 // reduction).  With VEC (N a multiple of 4, aligned rows) the states of the next kStepAhead - 1
 // groups are on their way into the thread's own slots of shared memory, and the next group's
-// inputs into registers, while one group is computed.
+// inputs into registers, while one group is computed.  256 sequences of 8192 bf16 channels, 16
+// states: 64 us, 4.4 TB/s; every lane forming softplus and gate for itself, one sequence at a time,
+// took 104 us, and 3 or 4 blocks of 256 threads per SM, which spill, 88 and 127 us.
 constexpr int kStepThreads = 128, kStepAhead = 2, kStepBatch = 16;
 
 template <class T, bool VEC, int LPC>
