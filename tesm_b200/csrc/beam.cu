@@ -507,6 +507,13 @@ __global__ void __launch_bounds__(kReorderThreads)
   }
 }
 
+// The widest access that all rows of a state are aligned to.
+static uint32_t state_vec(const tesm_b200_state_rows &s) {
+  const uint64_t bits = (uintptr_t)s.src | (uintptr_t)s.dst | (uint64_t)s.src_stride | (uint64_t)s.dst_stride |
+                        (uint64_t)s.row_bytes;
+  return bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : bits % 2 == 0 ? 2 : 1;
+}
+
 }  // namespace tesm
 
 extern "C" int tesm_b200_beam_select_workspace(int dtype, int64_t G, int64_t W, int64_t V, int64_t K, int64_t *bytes_out) {
@@ -571,6 +578,9 @@ extern "C" int tesm_b200_reorder_states(const tesm_b200_state_rows *states, int6
     TESM_REQUIRE(s.src_stride >= s.row_bytes && s.dst_stride >= s.row_bytes, "reorder_states: rows overlap");
     TESM_REQUIRE(s.src != s.dst || (Win == Wout && s.src_stride == s.dst_stride),
                  "reorder_states: in place needs as many beams out as in");
+    const uint64_t cols = (uint64_t)s.row_bytes / state_vec(s);
+    if (cols >= (1ull << 32) || (uint64_t)G >= (1ull << 32) || (uint64_t)G * cols >= (1ull << 32))
+      return fail(TESM_EUNSUPPORTED, "reorder_states: a state of 2^32 columns or more");
     const char *lo = (const char *)s.dst, *hi = lo + (G * Wout - 1) * s.dst_stride + s.row_bytes;
     TESM_REQUIRE((const char *)(parents + G * Wout) <= lo || (const char *)parents >= hi,
                  "reorder_states: parents lie inside a state");
@@ -593,12 +603,8 @@ extern "C" int tesm_b200_reorder_states(const tesm_b200_state_rows *states, int6
     }
     if (i == n || states[i].row_bytes == 0) continue;
     const tesm_b200_state_rows &s = states[i];
-    const uint64_t bits = (uintptr_t)s.src | (uintptr_t)s.dst | (uint64_t)s.src_stride | (uint64_t)s.dst_stride |
-                          (uint64_t)s.row_bytes;
-    const uint32_t vec = bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : bits % 2 == 0 ? 2 : 1;
+    const uint32_t vec = state_vec(s);
     const uint64_t cols = (uint64_t)s.row_bytes / vec;
-    if (cols >= (1ull << 32) || (uint64_t)G * cols >= (1ull << 32))
-      return fail(TESM_EUNSUPPORTED, "reorder_states: a state of 2^32 columns or more");
     t.d[t.n] = StateDesc{(const char *)s.src, (char *)s.dst, s.src_stride, s.dst_stride, (uint32_t)cols,
                          (uint32_t)blocks, vec};
     blocks += (uint64_t)ceil_div(G * (int64_t)cols, kReorderThreads);

@@ -65,6 +65,13 @@ def test_reorder_refuses_parents_inside_a_state(parents):
     assert "parents" in _lib.last_error()
 
 
+def test_reorder_checks_every_state_before_the_first_launch():
+    """200 states take two launches; a size that only the last one refuses refuses the call."""
+    good, bad = (4096, 4096, 64, 64, 64), (4096, 4096, 1 << 36, 1 << 36, 1 << 36)
+    t = rows(*[good] * 199, bad)
+    assert status("tesm_b200_reorder_states", ctypes.addressof(t), 200, 2, 4, 4, ctypes.c_void_p(1 << 60), None) == 5
+
+
 def test_reorder_refuses_no_table():
     assert status("tesm_b200_reorder_states", None, 1, 2, 4, 4, P, None) == 1
     assert status("tesm_b200_reorder_states", None, 0, 2, 4, 4, P, None) == 0
