@@ -386,11 +386,14 @@ int tesm_b200_causal_conv(const void *x, int dtype, int64_t ldxb, int64_t ldxl, 
  * element strides (batch, token) of x, dt, bm, cm, z, out.  A (D, N), skip (D), dt_bias (D) fp32, the
  * last two nullable.  state (B, D, N) fp32, dense, nullable: the state before the first token
  * (zeros without it), replaced by the one after the last.  lengths as in tesm_b200_causal_conv.  out
- * must not overlap the inputs.  1 <= N <= 128; states and sums in fp32. */
+ * must not overlap the inputs, nor state anything.  1 <= N <= 128; states and sums in fp32.  ws:
+ * 16-byte aligned scratch of tesm_b200_ssm_scan_workspace bytes (0 for most shapes: long sequences of
+ * few channels run in two launches), free again once the work has run on the stream. */
 int tesm_b200_ssm_scan(const void *x, const void *dt, const void *bm, const void *cm, const void *z, void *out,
                        const int64_t *strides, int dtype, int64_t B, int64_t L, int64_t D, int64_t N, const float *A,
                        const float *skip, const float *dt_bias, int softplus, float *state, const int32_t *lengths,
-                       tesm_stream_t stream);
+                       void *ws, int64_t ws_bytes, tesm_stream_t stream);
+int tesm_b200_ssm_scan_workspace(int64_t B, int64_t L, int64_t D, int64_t N, int64_t *bytes_out);
 
 #ifdef __cplusplus
 }

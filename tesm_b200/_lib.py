@@ -88,7 +88,8 @@ SIGNATURES = {
     "tesm_b200_causal_conv": [c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_int,
                               c_vp, c_i64, c_i64, c_vp],
     "tesm_b200_ssm_scan": [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp,
-                           c_vp, c_int, c_vp, c_vp, c_vp],
+                           c_vp, c_int, c_vp, c_vp, c_vp, c_i64, c_vp],
+    "tesm_b200_ssm_scan_workspace": [c_i64, c_i64, c_i64, c_i64, c_vp],
 }
 _RESTYPES = {"tesm_b200_last_error": ctypes.c_char_p}
 
@@ -137,7 +138,7 @@ def check(status: int, what: str):
 # number of entry-point calls that enqueue device work (bench.py reports it as gpu_launches)
 launch_count = 0
 _NO_LAUNCH = {"tesm_b200_version", "tesm_b200_last_error", "tesm_b200_device_status", "tesm_b200_scan_workspace",
-              "tesm_b200_beam_select_workspace"}
+              "tesm_b200_beam_select_workspace", "tesm_b200_ssm_scan_workspace"}
 
 
 def call(name: str, *args):

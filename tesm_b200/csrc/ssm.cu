@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(kConvThreads)
   }
 }
 
-// ------------------------------------------------------------ selective scan, prompts: lanes share the states
+// ------------------------------------------------------------ selective scan, prompts
 // h_t = exp(dt_t A) h_{t-1} + (dt_t x_t) B_t,  y_t = C_t . h_t + D x_t,  out = y silu(z).
 // A channel's N states are spread over LPC lanes with NPT states each (zero-padded to NPT * LPC),
 // which walk the sequence in double groups of 2 LPC tokens.  Lane q loads tokens q and LPC + q of
@@ -283,7 +283,12 @@ __global__ void __launch_bounds__(kConvThreads)
 // SM), but the 9 instructions per state, at 0.4 of the issue rate with the 7 warps that an SM
 // gets from one sequence; four sequences of 2048 tokens, twice the work, take 506 us.  Inputs staged
 // through shared memory with softplus formed by the loading thread took 354 us; 16 instead of 32
-// tokens ahead 368 us; two states per lane (twice the warps, narrower row accesses) 541 us.
+// tokens ahead 368 us; two states per lane (twice the warps, narrower row accesses) 541 us; lanes
+// that share the tokens instead, joined by shuffles, 394 us.
+// Few channels leave schedulers without a warp: their sequences are cut into segments (a.segs > 1).
+// A first launch (ENDS) runs all but the last segment from zero, without outputs, and leaves their
+// end states and sums of dt; the second starts each segment from the state that these lead to, since
+// the decay over a segment is exp(A sum dt).
 template <class T>
 struct ScanArgs {
   Rows<const T> x, dt, bm, cm, z;
@@ -291,8 +296,20 @@ struct ScanArgs {
   const float *A, *skip, *dt_bias;
   float *state;
   const int *lengths;
-  int L, D, N, softplus, vec_rows, vec_bc, chunks;
+  int L, D, N, softplus, vec_bc, chunks;
+  // sequences cut into segments of seg tokens (k_ssm_scan): the state at the start of the first, and
+  // for each but the last its end state from zero (of the first: from that start) and its sum of dt
+  int segs, seg;
+  int64_t rows;  // batch * channels
+  float *start, *ends, *sums;
 };
+
+// The hardware exponential is 2e-8 too small on average where decays matter (arguments of -0.001 to
+// -0.5), which a state adds up over as many tokens as it remembers.  2^2.9e-8 puts that back in the
+// FMA that forms the argument: mean error 2e-9 instead of -2e-8, states of 73 to 4000 tokens off by
+// 2e-7 to 6e-7 instead of 5e-7 to 15e-7 (relative norm; 6e-7 with expf).  A step of 0 still decays by
+// exactly 1, to which 2^2.9e-8 rounds.
+constexpr float kEx2Shift = 2.9e-8f;
 
 constexpr int kScanThreads = 128, kScanAhead = 32;
 
@@ -310,7 +327,16 @@ struct ScanShape {
   static constexpr int BLOCKS = NP > 16 ? 2 : 4;    // per SM that the registers allow: 16 states, 4 sequences: 506 us, with 2 blocks 631
 };
 
-template <class T, int NPT, int LPC>
+// h 2^e for the e of a whole segment.  Token by token a state that is 0 or infinite stays so, and one
+// that underflows or overflows halfway to its value does not exist: hence four steps, each of which
+// stays in range where the result does.
+__device__ __forceinline__ float decayed(float h, float e) {
+  if (h == 0.f || isinf(h)) return h;
+  const float f = ex2_approx(0.25f * e);
+  return h * f * f * f * f;
+}
+
+template <class T, int NPT, int LPC, bool ENDS>
 __global__ void __launch_bounds__(kScanThreads, ScanShape<NPT, LPC>::BLOCKS) k_ssm_scan(const __grid_constant__ ScanArgs<T> a) {
   using S = ScanShape<NPT, LPC>;
   constexpr int NP = S::NP, CT = S::CT, TT = S::TT, BV = S::BV, BIPT = S::BIPT, PF = S::PF, G = S::G;
@@ -321,25 +347,39 @@ __global__ void __launch_bounds__(kScanThreads, ScanShape<NPT, LPC>::BLOCKS) k_s
   pdl_trigger();
   pdl_wait();
   const int tid = threadIdx.x;
-  const int64_t b = blockIdx.x / a.chunks;
+  const int B = (int)(a.rows / a.D);
+  const int s = blockIdx.x / a.chunks / B;
+  const int64_t b = blockIdx.x / a.chunks % B;
   const int c = (int)(blockIdx.x % a.chunks) * CT + tid / LPC;
   const int q = tid % LPC, n0 = q * NPT;
-  const int T_b = seq_len(a.lengths, b, a.L);
+  const int t_lo = s * a.seg, len = seq_len(a.lengths, b, a.L), T_b = min(len, t_lo + a.seg);
   const bool live = c < a.D;
+  const int64_t at0 = (b * a.D + c) * (int64_t)a.N + n0, all = a.rows * a.N;
 
   float A2[NPT], h[NPT];
 #pragma unroll
   for (int i = 0; i < NPT; ++i) {
-    const int64_t at = (int64_t)c * a.N + n0 + i;
     const bool on = live && n0 + i < a.N;
-    A2[i] = on ? a.A[at] * kLog2e : 0.f;
-    h[i] = on && a.state ? a.state[b * (int64_t)a.D * a.N + at] : 0.f;
+    const float A = on ? a.A[(int64_t)c * a.N + n0 + i] * kLog2e : 0.f;
+    A2[i] = isinf(A) ? copysignf(3.4e38f, A) : A;  // times the 0 of a token behind the end: 0, not NaN
+    h[i] = 0.f;
+    if (!on) continue;
+    if constexpr (ENDS) {
+      if (s == 0 && a.state) a.start[at0 + i] = h[i] = a.state[at0 + i];
+    } else if (s == 0) {
+      if (a.state) h[i] = a.segs > 1 ? a.start[at0 + i] : a.state[at0 + i];
+    } else {
+      h[i] = a.ends[at0 + i];
+      for (int e = 1; e < s; ++e)
+        h[i] = decayed(h[i], a.sums[e * a.rows + b * a.D + c] * A2[i]) + a.ends[e * all + at0 + i];
+    }
   }
+  float dsum = 0.f;
   const float bias = live && a.dt_bias ? a.dt_bias[c] : 0.f, skip = live && a.skip ? a.skip[c] : 0.f;
 
   // this lane's rows: tokens q, q + LPC, ...
-  const T *px = a.x.at(b, q, c), *pd = a.dt.at(b, q, c), *pz = a.z.p ? a.z.at(b, q, c) : px;
-  T *po = a.out.at(b, q, c);
+  const T *px = a.x.at(b, t_lo + q, c), *pd = a.dt.at(b, t_lo + q, c), *pz = a.z.p ? a.z.at(b, t_lo + q, c) : px;
+  T *po = a.out.at(b, t_lo + q, c);
   const int64_t sx = LPC * a.x.ldl, sd = LPC * a.dt.ldl, sz = LPC * (a.z.p ? a.z.ldl : a.x.ldl), so = LPC * a.out.ldl;
   const int mine = live ? T_b - q : 0;  // a group that starts at t holds a token of this lane if t < mine
   T nx[PF][2], nd[PF][2], nz[PF][2];
@@ -349,8 +389,8 @@ __global__ void __launch_bounds__(kScanThreads, ScanShape<NPT, LPC>::BLOCKS) k_s
       const bool on = t + w * LPC < mine;
       nx[k][w] = on ? *px : from_f<T>(0.f);
       nd[k][w] = on ? *pd : from_f<T>(0.f);
-      nz[k][w] = on ? *pz : from_f<T>(0.f);
-      px += sx, pd += sd, pz += sz;
+      if constexpr (!ENDS) nz[k][w] = on ? *pz : from_f<T>(0.f), pz += sz;
+      px += sx, pd += sd;
     }
   };
   Pack<T, BV> nb[BIPT], nc[BIPT];
@@ -360,20 +400,23 @@ __global__ void __launch_bounds__(kScanThreads, ScanShape<NPT, LPC>::BLOCKS) k_s
       const int it = tid + i * kScanThreads, t = t0 + it / (NP / BV), n = it % (NP / BV) * BV;
       const int have = it < S::BITEMS && t < T_b ? a.N - n : 0;
       nb[i].load(a.bm.at(b, t, n), a.vec_bc, have);
-      nc[i].load(a.cm.at(b, t, n), a.vec_bc, have);
+      if constexpr (!ENDS) nc[i].load(a.cm.at(b, t, n), a.vec_bc, have);
     }
   };
 #pragma unroll
-  for (int k = 0; k < PF; ++k) fetch(k, k * G);
-  fetch_bc(0);
-  for (int t0 = 0; t0 < T_b; t0 += TT) {
-    if (t0) __syncthreads();  // the tile before has been read
+  for (int k = 0; k < PF; ++k) fetch(k, t_lo + k * G);
+  fetch_bc(t_lo);
+  for (int t0 = t_lo; t0 < T_b; t0 += TT) {
+    if (t0 > t_lo) __syncthreads();  // the tile before has been read
 #pragma unroll
     for (int i = 0; i < BIPT; ++i) {
       const int it = tid + i * kScanThreads, at = it / (NP / BV) * NP + it % (NP / BV) * BV;
       if (it < S::BITEMS) {
 #pragma unroll
-        for (int e = 0; e < BV; ++e) sb[at + e] = to_f(nb[i].v[e]), sc[at + e] = to_f(nc[i].v[e]);
+        for (int e = 0; e < BV; ++e) {
+          sb[at + e] = to_f(nb[i].v[e]);
+          if constexpr (!ENDS) sc[at + e] = to_f(nc[i].v[e]);
+        }
       }
     }
     __syncthreads();
@@ -383,12 +426,14 @@ __global__ void __launch_bounds__(kScanThreads, ScanShape<NPT, LPC>::BLOCKS) k_s
 #pragma unroll
       for (int k = 0; k < PF; ++k) {
         const int t = t0 + g + k * G;
-        const float2 x = make_float2(to_f(nx[k][0]), to_f(nx[k][1])), z = make_float2(to_f(nz[k][0]), to_f(nz[k][1]));
+        const float2 x = make_float2(to_f(nx[k][0]), to_f(nx[k][1]));
+        const float2 z = ENDS ? x : make_float2(to_f(nz[k][0]), to_f(nz[k][1]));
         float2 d = __fadd2_rn(make_float2(to_f(nd[k][0]), to_f(nd[k][1])), make_float2(bias, bias));
         fetch(k, t + PF * G);
         if (a.softplus) d = softplus2(d);
         const bool on0 = t < mine, on1 = t + LPC < mine;
         d = make_float2(on0 ? d.x : 0.f, on1 ? d.y : 0.f);  // behind the end: a = 1, no input
+        if constexpr (ENDS) dsum += d.x + d.y;
         const float2 u = __fmul2_rn(d, x);
         float ys[2];
 #pragma unroll
@@ -400,38 +445,43 @@ __global__ void __launch_bounds__(kScanThreads, ScanShape<NPT, LPC>::BLOCKS) k_s
             const float uj = __shfl_sync(0xffffffffu, w ? u.y : u.x, j, LPC);
             const float *bp = sb + (g + k * G + w * LPC + j) * NP + n0, *cp = sc + (g + k * G + w * LPC + j) * NP + n0;
             if constexpr (NPT == 1) {
-              h[0] = fmaf(ex2_approx(dj * A2[0]), h[0], uj * bp[0]);
-              p[j] = cp[0] * h[0];
+              h[0] = fmaf(ex2_approx(fmaf(dj, A2[0], kEx2Shift)), h[0], uj * bp[0]);
+              if constexpr (!ENDS) p[j] = cp[0] * h[0];
             } else {
               const float2 d2 = make_float2(dj, dj), u2 = make_float2(uj, uj);
               Pack<float, NPT> Bv, Cv;
               Bv.load_all(bp);
-              Cv.load_all(cp);
+              if constexpr (!ENDS) Cv.load_all(cp);
               float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
               for (int i = 0; i < H; ++i) {
-                const float2 e = __fmul2_rn(d2, make_float2(A2[2 * i], A2[2 * i + 1]));
+                const float2 e = __ffma2_rn(d2, make_float2(A2[2 * i], A2[2 * i + 1]), make_float2(kEx2Shift, kEx2Shift));
                 float2 hv = make_float2(h[2 * i], h[2 * i + 1]);
                 hv = __ffma2_rn(make_float2(ex2_approx(e.x), ex2_approx(e.y)), hv,
                                 __fmul2_rn(u2, make_float2(Bv.v[2 * i], Bv.v[2 * i + 1])));
                 h[2 * i] = hv.x, h[2 * i + 1] = hv.y;
-                const float2 C2 = make_float2(Cv.v[2 * i], Cv.v[2 * i + 1]);
-                acc = i ? __ffma2_rn(C2, hv, acc) : __fmul2_rn(C2, hv);
+                if constexpr (!ENDS) {
+                  const float2 C2 = make_float2(Cv.v[2 * i], Cv.v[2 * i + 1]);
+                  acc = i ? __ffma2_rn(C2, hv, acc) : __fmul2_rn(C2, hv);
+                }
               }
-              p[j] = acc.x + acc.y;
+              if constexpr (!ENDS) p[j] = acc.x + acc.y;
             }
           }
+          if constexpr (!ENDS) {
 #pragma unroll
-          for (int o = LPC / 2; o; o >>= 1) {
-            const bool up = q & o;
+            for (int o = LPC / 2; o; o >>= 1) {
+              const bool up = q & o;
 #pragma unroll
-            for (int j = 0; j < o; ++j) {
-              const float keep = up ? p[j + o] : p[j], give = up ? p[j] : p[j + o];
-              p[j] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+              for (int j = 0; j < o; ++j) {
+                const float keep = up ? p[j + o] : p[j], give = up ? p[j] : p[j + o];
+                p[j] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+              }
             }
+            ys[w] = p[0];
           }
-          ys[w] = p[0];
         }
+        if constexpr (ENDS) continue;
         float2 y = __ffma2_rn(make_float2(skip, skip), x, make_float2(ys[0], ys[1]));
         if (a.z.p) y = __fmul2_rn(y, silu2(z));
         if (on0) *po = from_f<T>(y.x);
@@ -441,250 +491,23 @@ __global__ void __launch_bounds__(kScanThreads, ScanShape<NPT, LPC>::BLOCKS) k_s
       }
     }
   }
-  if (live) {  // outputs behind the end are zeros
-    for (int t = T_b + q; t < a.L; t += LPC) *a.out.at(b, t, c) = from_f<T>(0.f);
-  }
-  if (a.state && live && T_b > 0) {
+  if constexpr (ENDS) {
+#pragma unroll
+    for (int o = 1; o < LPC; o <<= 1) dsum += __shfl_xor_sync(0xffffffffu, dsum, o);
+    if (live && q == 0) a.sums[s * a.rows + b * a.D + c] = dsum;
 #pragma unroll
     for (int i = 0; i < NPT; ++i)
-      if (n0 + i < a.N) a.state[(b * a.D + c) * (int64_t)a.N + n0 + i] = h[i];
+      if (live && n0 + i < a.N) a.ends[s * all + at0 + i] = h[i];
+    return;
   }
-}
-
-// ------------------------------------------------------------ selective scan, prompts: lanes share the tokens
-// For sequences with few channels, whose tokens one after the other would leave most of the
-// schedulers without a warp.  A lane owns two channels (packed arithmetic) and kTimeItems
-// consecutive tokens, 32 lanes a tile of 32 * kTimeItems tokens.  For each state the lane first runs
-// its tokens from zero, the lanes join their (decay, end state) pairs in five shuffle rounds,
-// then the lane runs its tokens again from the state that reaches it: the exponentials are
-// taken once and kept for both runs.  Two states at a time, for two independent chains.  B and C
-// are staged in fp32 for chunks of 16 states (any N), x, dt and z as planes of channel pairs; the
-// next tile's rows are loaded while one is computed.
-// One bf16 sequence of 8192 tokens, 2048 channels, 16 states: 226 us, against 532 us of the kernel
-// above; at 8192 channels 394 us against 340.  It issues 12 instructions per state at 0.4 of
-// the rate: 7 warps per SM, held back by the shuffle rounds (a fifth of the time).
-constexpr int kTimeItems = 8, kTimeStates = 16, kTimePairs = 4;  // tokens per lane; states per chunk; warps per block
-
-template <class T>
-struct TimeShape {
-  static constexpr int I = kTimeItems, TT = 32 * I, CH = 2 * kTimePairs, THREADS = 32 * kTimePairs;
-  // planes of one channel pair, [I][ROW]: rows 4 words apart modulo 32, for the staging stores (lanes along I)
-  static constexpr int ROW = 32 + 4, PITCH = I * ROW;
-  // planes of one state, [I / 2][BROW] of two items' values
-  static constexpr int BROW = 2 * 32 + 8, BPLANE = I / 2 * BROW, BC = kTimeStates * BPLANE;
-  static constexpr int XIT = TT / THREADS, BIT = TT * (kTimeStates / 8) / THREADS;  // accesses per thread and tile
-  static int smem(int N) { return 4 * (2 * BC + 4 * ((N + 1) & ~1) * kTimePairs) + 3 * 2 * (int)sizeof(T) * kTimePairs * PITCH; }
-};
-
-template <class T>
-struct alignas(2 * sizeof(T)) Pair {
-  T a, b;
-  __device__ __forceinline__ float2 f() const { return make_float2(to_f(a), to_f(b)); }
-};
-
-template <class T>
-__global__ void __launch_bounds__(TimeShape<T>::THREADS, 1) k_ssm_scan_time(const __grid_constant__ ScanArgs<T> a) {
-  using S = TimeShape<T>;
-  constexpr int I = S::I, TT = S::TT, CH = S::CH, ROW = S::ROW, PITCH = S::PITCH, BROW = S::BROW, BPLANE = S::BPLANE;
-  constexpr int THREADS = S::THREADS, XIT = S::XIT, BIT = S::BIT, NC = kTimeStates, PAIRS = kTimePairs;
-  static_assert(CH == 8 && TT % THREADS == 0, "one access of 8 channels per token");
-  extern __shared__ __align__(16) float smem[];
-  const int Np = (a.N + 1) & ~1;                                // states two at a time: zeros behind the last
-  float *sb = smem, *sc = sb + S::BC;                           // [NC][I / 2][BROW]
-  float2 *sa = reinterpret_cast<float2 *>(sc + S::BC);          // [Np][PAIRS] A log2(e)
-  float2 *sh = sa + Np * PAIRS;                                 // [Np][PAIRS] state at the tile's start
-  Pair<T> *sx = reinterpret_cast<Pair<T> *>(sh + Np * PAIRS);   // [PAIRS][I][ROW]
-  Pair<T> *sd = sx + PAIRS * PITCH, *sz = sd + PAIRS * PITCH;
-  pdl_trigger();
-  pdl_wait();
-  const int tid = threadIdx.x, tl = tid & 31, pair = tid >> 5;
-  const int64_t b = blockIdx.x / a.chunks;
-  const int c0 = (int)(blockIdx.x % a.chunks) * CH, c = c0 + 2 * pair;
-  const int T_b = seq_len(a.lengths, b, a.L);
-  const int live = min(2, a.D - c);  // channels of this warp's pair that exist
-  float *state = a.state ? a.state + (b * a.D + c) * (int64_t)a.N : nullptr;
-
-  for (int n = tl; n < Np; n += 32) {
-    float2 A = make_float2(0.f, 0.f), h = A;
-    const int64_t at = (int64_t)c * a.N + n;
-    if (n < a.N && live > 0) A.x = a.A[at] * kLog2e, h.x = state ? state[n] : 0.f;
-    if (n < a.N && live > 1) A.y = a.A[at + a.N] * kLog2e, h.y = state ? state[a.N + n] : 0.f;
-    sa[n * PAIRS + pair] = A;
-    sh[n * PAIRS + pair] = h;
+  if (live) {  // outputs behind the end are zeros
+    const int t_hi = min(a.L, t_lo + a.seg);
+    for (int t = max(len, t_lo) + q; t < t_hi; t += LPC) *a.out.at(b, t, c) = from_f<T>(0.f);
   }
-  const float2 bias = make_float2(a.dt_bias && live > 0 ? a.dt_bias[c] : 0.f, a.dt_bias && live > 1 ? a.dt_bias[c + 1] : 0.f);
-  const float2 skip = make_float2(a.skip && live > 0 ? a.skip[c] : 0.f, a.skip && live > 1 ? a.skip[c + 1] : 0.f);
-
-  Pack<T, CH> px[XIT], pd[XIT], pz[XIT];
-  Pack<T, 8> pb[BIT], pc[BIT];
-  auto fetch_rows = [&](int t0) {
+  if (a.state && live && len > 0 && s == a.segs - 1) {
 #pragma unroll
-    for (int k = 0; k < XIT; ++k) {
-      const int t = t0 + tid + k * THREADS, have = t < T_b ? a.D - c0 : 0;
-      px[k].load(a.x.at(b, t, c0), a.vec_rows, have);
-      pd[k].load(a.dt.at(b, t, c0), a.vec_rows, have);
-      if (a.z.p) pz[k].load(a.z.at(b, t, c0), a.vec_rows, have);
-    }
-  };
-  auto fetch_bc = [&](int t0, int n0) {
-#pragma unroll
-    for (int k = 0; k < BIT; ++k) {
-      const int it = tid + k * THREADS, t = t0 + it % TT, n = n0 + it / TT * 8;
-      const int have = t < T_b ? a.N - n : 0;
-      pb[k].load(a.bm.at(b, t, n), a.vec_bc, have);
-      pc[k].load(a.cm.at(b, t, n), a.vec_bc, have);
-    }
-  };
-  fetch_rows(0);
-  fetch_bc(0, 0);
-  for (int t0 = 0; t0 < T_b; t0 += TT) {
-    __syncthreads();  // the rows of the tile before have been stored
-    // rows -> planes; token t of the tile is item t % I of lane t / I
-#pragma unroll
-    for (int k = 0; k < XIT; ++k) {
-      const int r = tid + k * THREADS, at = r % I * ROW + r / I;
-#pragma unroll
-      for (int e = 0; e < PAIRS; ++e) {
-        sx[at + e * PITCH] = Pair<T>{px[k].v[2 * e], px[k].v[2 * e + 1]};
-        sd[at + e * PITCH] = Pair<T>{pd[k].v[2 * e], pd[k].v[2 * e + 1]};
-        if (a.z.p) sz[at + e * PITCH] = Pair<T>{pz[k].v[2 * e], pz[k].v[2 * e + 1]};
-      }
-    }
-    float2 dt[I], u[I], y[I];
-    for (int n0 = 0; n0 < a.N; n0 += NC) {
-      if (n0) __syncthreads();  // the chunk before has been read
-#pragma unroll
-      for (int k = 0; k < BIT; ++k) {
-        const int it = tid + k * THREADS, r = it % TT, n = it / TT * 8, i = r % I, l = r / I;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int at = (n + e) * BPLANE + i / 2 * BROW + l * 2 + i % 2;
-          sb[at] = to_f(pb[k].v[e]);
-          sc[at] = to_f(pc[k].v[e]);
-        }
-      }
-      __syncthreads();
-      if (n0 + NC < a.N) fetch_bc(t0, n0 + NC);
-      else fetch_bc(t0 + TT, 0);
-      if (n0 == 0) {
-        fetch_rows(t0 + TT);
-#pragma unroll
-        for (int i = 0; i < I; ++i) {
-          const int at = pair * PITCH + i * ROW + tl;
-          const float2 x = sx[at].f();
-          float2 d = __fadd2_rn(sd[at].f(), bias);
-          if (a.softplus) d = softplus2(d);
-          if (t0 + tl * I + i >= T_b) d = make_float2(0.f, 0.f);  // behind the end: a = 1, no input
-          dt[i] = d;
-          u[i] = __fmul2_rn(d, x);
-          y[i] = __fmul2_rn(skip, x);
-        }
-      }
-      const int nn = min(NC, Np - n0);
-      auto values = [&](const float *p, int n, int i) {  // of items i, i + 1
-        return reinterpret_cast<const float2 *>(p)[(n * BPLANE + i / 2 * BROW) / 2 + tl];
-      };
-#pragma unroll 1
-      for (int n = 0; n < nn; n += 2) {
-        float2 A[2], start[2], ea[2][I], in[2][I], h[2], P[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          A[k] = sa[(n0 + n + k) * PAIRS + pair];
-          start[k] = sh[(n0 + n + k) * PAIRS + pair];
-        }
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int i = 0; i < I; i += 2) {
-            const float2 B2 = values(sb, n + k, i);
-            in[k][i] = __fmul2_rn(u[i], make_float2(B2.x, B2.x));
-            in[k][i + 1] = __fmul2_rn(u[i + 1], make_float2(B2.y, B2.y));
-          }
-#pragma unroll
-        for (int i = 0; i < I; ++i)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float2 e = __fmul2_rn(dt[i], A[k]);
-            ea[k][i] = make_float2(ex2_approx(e.x), ex2_approx(e.y));
-          }
-        // this lane's tokens from zero (the first lane: from the tile's state), and its decay
-#pragma unroll
-        for (int k = 0; k < 2; ++k) h[k] = in[k][0], P[k] = ea[k][0];
-        if (tl == 0) {
-#pragma unroll
-          for (int k = 0; k < 2; ++k) h[k] = __ffma2_rn(ea[k][0], start[k], h[k]);
-        }
-#pragma unroll
-        for (int i = 1; i < I; ++i)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            h[k] = __ffma2_rn(ea[k][i], h[k], in[k][i]);
-            P[k] = __fmul2_rn(P[k], ea[k][i]);
-          }
-        if (tl == 0) {  // nothing lies before it; lanes that reach it take over its 0, so that no round needs a test
-#pragma unroll
-          for (int k = 0; k < 2; ++k) P[k] = make_float2(0.f, 0.f);
-        }
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float2 hu = make_float2(__shfl_up_sync(0xffffffffu, h[k].x, o), __shfl_up_sync(0xffffffffu, h[k].y, o));
-            h[k] = __ffma2_rn(P[k], hu, h[k]);
-            if (o < 16)
-              P[k] = __fmul2_rn(P[k], make_float2(__shfl_up_sync(0xffffffffu, P[k].x, o), __shfl_up_sync(0xffffffffu, P[k].y, o)));
-          }
-        float2 g[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          g[k] = make_float2(__shfl_up_sync(0xffffffffu, h[k].x, 1), __shfl_up_sync(0xffffffffu, h[k].y, 1));
-          if (tl == 0) g[k] = start[k];
-        }
-#pragma unroll
-        for (int i = 0; i < I; i += 2)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float2 C2 = values(sc, n + k, i);
-            g[k] = __ffma2_rn(ea[k][i], g[k], in[k][i]);
-            y[i] = __ffma2_rn(make_float2(C2.x, C2.x), g[k], y[i]);
-            g[k] = __ffma2_rn(ea[k][i + 1], g[k], in[k][i + 1]);
-            y[i + 1] = __ffma2_rn(make_float2(C2.y, C2.y), g[k], y[i + 1]);
-          }
-        if (tl == 31) {
-#pragma unroll
-          for (int k = 0; k < 2; ++k) sh[(n0 + n + k) * PAIRS + pair] = h[k];
-        }
-      }
-    }
-    // gate, then back through the planes of x into rows
-#pragma unroll
-    for (int i = 0; i < I; ++i) {
-      const int at = pair * PITCH + i * ROW + tl;
-      float2 o = y[i];
-      if (a.z.p) o = __fmul2_rn(o, silu2(sz[at].f()));
-      sx[at] = Pair<T>{from_f<T>(o.x), from_f<T>(o.y)};
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < XIT; ++k) {
-      const int r = tid + k * THREADS, at = r % I * ROW + r / I;
-      if (t0 + r >= T_b) continue;
-      Pack<T, CH> o;
-#pragma unroll
-      for (int e = 0; e < PAIRS; ++e) o.v[2 * e] = sx[at + e * PITCH].a, o.v[2 * e + 1] = sx[at + e * PITCH].b;
-      o.store(a.out.at(b, t0 + r, c0), a.vec_rows, a.D - c0);
-    }
-  }
-  Pack<T, CH> zero;  // outputs behind the end
-  zero.zero();
-  for (int t = T_b + tid; t < a.L; t += THREADS) zero.store(a.out.at(b, t, c0), a.vec_rows, a.D - c0);
-  if (state && T_b > 0) {
-    __syncwarp();
-    for (int n = tl; n < a.N; n += 32) {
-      const float2 h = sh[n * PAIRS + pair];
-      if (live > 0) state[n] = h.x;
-      if (live > 1) state[a.N + n] = h.y;
-    }
+    for (int i = 0; i < NPT; ++i)
+      if (n0 + i < a.N) a.state[at0 + i] = h[i];
   }
 }
 
@@ -797,7 +620,7 @@ __global__ void __launch_bounds__(kStepThreads, 5) k_ssm_step(const __grid_const
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         // a sequence without a token may hold anything in its row of B and C
-        h.v[i] = fmaf(ex2_approx(dr * A.v[i]), h.v[i], ur * to_f(in.bm[r].v[i]));
+        h.v[i] = fmaf(ex2_approx(fmaf(dr, A.v[i], kEx2Shift)), h.v[i], ur * to_f(in.bm[r].v[i]));
         y[r] = fmaf(to_f(in.cm[r].v[i]), h.v[i], y[r]);
       }
       if (st) {
@@ -845,7 +668,11 @@ template <class T, int NPT, int LPC>
 static int launch_scan(ScanArgs<T> a, int64_t B, cudaStream_t st) {
   using S = ScanShape<NPT, LPC>;
   a.chunks = (int)ceil_div(a.D, S::CT);
-  return launch_scan_k(k_ssm_scan<T, NPT, LPC>, a, B * a.chunks, kScanThreads, S::SMEM, st);
+  if (a.segs > 1) {
+    const int rc = launch_scan_k(k_ssm_scan<T, NPT, LPC, true>, a, B * a.chunks * (a.segs - 1), kScanThreads, S::SMEM, st);
+    if (rc) return rc;
+  }
+  return launch_scan_k(k_ssm_scan<T, NPT, LPC, false>, a, B * a.chunks * a.segs, kScanThreads, S::SMEM, st);
 }
 
 template <class T, int LPC>
@@ -857,10 +684,33 @@ static int launch_step(ScanArgs<T> a, int64_t B, cudaStream_t st) {
              : launch_k("ssm_scan", k_ssm_step<T, false, LPC>, grid, block, 0, st, a, (int)B);
 }
 
-template <class T>
-static int ssm_scan_t(ScanArgs<T> a, int64_t B, cudaStream_t st) {
+static int pad_states(int64_t N) {
   int np = 1;
-  while (np < a.N) np <<= 1;
+  while (np < N) np <<= 1;
+  return np;
+}
+
+// Tokens per segment.  A warp's step takes about 65 ns however few warps there are, and 36 ns of its
+// scheduler where there are many; a second pass adds 22.  So with under one warp per scheduler
+// cutting the sequences wins (8192 tokens, 2048 channels, 16 states: 544 us whole, 281 in 4, 248 in 8, 219
+// in 16 segments; 512 tokens: 22 in 4, 29 whole).  At 7 warps per 8 schedulers it is about even (4096
+// channels: 119 us in 16 segments, 108 whole at 2048 tokens, 227 and 266 at 4096, whose inputs
+// leave L2) and above it loses (8192 channels: 341 us whole, 402 in 2).  Segments have 128 tokens at
+// least, and under four of them do not pay for the second launch.
+static int64_t scan_segment(int64_t B, int64_t L, int64_t D, int64_t N) {
+  const int64_t warps = ceil_div(B * D * (int64_t)pad_states(N), 128);
+  const int64_t s = L / 128 < 16 ? L / 128 : 16;
+  return s < 4 || 2 * warps > 7 * (int64_t)sm_count() ? L : round_up(ceil_div(L, s), kScanAhead);
+}
+static int64_t scan_ws_floats(int64_t B, int64_t L, int64_t D, int64_t N) {
+  if (B == 0 || D == 0 || L <= 1) return 0;
+  const int64_t S = ceil_div(L, scan_segment(B, L, D, N));
+  return S > 1 ? S * B * D * N + (S - 1) * B * D : 0;
+}
+
+template <class T>
+static int ssm_scan_t(ScanArgs<T> a, int64_t B, float *ws, cudaStream_t st) {
+  const int np = pad_states(a.N);
   if (a.L == 1) {
     switch (np <= 4 ? 1 : np / 4) {
       case 1: return launch_step<T, 1>(a, B, st);
@@ -871,14 +721,12 @@ static int ssm_scan_t(ScanArgs<T> a, int64_t B, cudaStream_t st) {
       default: return launch_step<T, 32>(a, B, st);
     }
   }
-  // Warps of the kernel whose lanes share the states: 4 states per lane.  With fewer than there are
-  // schedulers the lanes share the tokens instead, where the sequences fill half a tile of them and
-  // the rows can be staged by 16-byte accesses (unaligned fp32 rows, 578 warps: 42 us against 29).
-  const int64_t warps = ceil_div(B * a.D * (int64_t)np, 128);
-  if (warps < 4 * (int64_t)sm_count() && a.L >= TimeShape<T>::TT / 2 && a.vec_rows) {
-    a.chunks = (int)ceil_div(a.D, TimeShape<T>::CH);
-    return launch_scan_k(k_ssm_scan_time<T>, a, B * a.chunks, TimeShape<T>::THREADS, TimeShape<T>::smem(a.N), st);
-  }
+  a.rows = B * a.D;
+  a.seg = (int)scan_segment(B, a.L, a.D, a.N);
+  a.segs = (int)ceil_div(a.L, a.seg);
+  a.start = ws;
+  a.ends = ws + a.rows * a.N;
+  a.sums = ws + a.segs * a.rows * a.N;
   switch (np) {
     case 1: return launch_scan<T, 1, 1>(a, B, st);
     case 2: return launch_scan<T, 2, 1>(a, B, st);
@@ -967,55 +815,65 @@ extern "C" int tesm_b200_causal_conv(const void *x, int dtype, int64_t ldxb, int
 namespace tesm {
 template <class T>
 static int ssm_scan_c(const void *x, const void *dt, const void *bm, const void *cm, const void *z, void *out,
-                      const int64_t *ld, int64_t B, ScanArgs<T> a, cudaStream_t st) {
+                      const int64_t *ld, int64_t B, ScanArgs<T> a, float *ws, cudaStream_t st) {
   a.x = {(const T *)x, ld[0], ld[1]};
   a.dt = {(const T *)dt, ld[2], ld[3]};
   a.bm = {(const T *)bm, ld[4], ld[5]};
   a.cm = {(const T *)cm, ld[6], ld[7]};
   a.z = {(const T *)z, ld[8], ld[9]};
   a.out = {(T *)out, ld[10], ld[11]};
-  uint64_t rows = (uintptr_t)x | (uintptr_t)dt | (uintptr_t)z | (uintptr_t)out;
   const int64_t es = sizeof(T);
-  for (int i : {0, 1, 2, 3, 10, 11}) rows |= (uint64_t)(ld[i] * es);
-  if (z) rows |= (uint64_t)(ld[8] * es) | (uint64_t)(ld[9] * es);
   uint64_t bc = (uintptr_t)bm | (uintptr_t)cm;
   for (int i : {4, 5, 6, 7}) bc |= (uint64_t)(ld[i] * es);
-  a.vec_rows = rows % 16 == 0;
   a.vec_bc = bc % 16 == 0;
-  return ssm_scan_t<T>(a, B, st);
+  return ssm_scan_t<T>(a, B, ws, st);
+}
+// Sizes of which no product leaves 64 bits and no grid 31.
+static bool scan_shape_ok(int64_t B, int64_t L, int64_t D) {
+  return B >= 0 && L >= 0 && D >= 0 && B < (1ll << 31) && L < (1ll << 30) && D < (1ll << 30) &&
+         B * ceil_div(D, 4) < (1ll << 31);
 }
 }  // namespace tesm
+
+extern "C" int tesm_b200_ssm_scan_workspace(int64_t B, int64_t L, int64_t D, int64_t N, int64_t *bytes_out) {
+  using namespace tesm;
+  TESM_REQUIRE(bytes_out && scan_shape_ok(B, L, D) && N >= 1 && N <= 128, "ssm_scan_workspace: bad shape");
+  *bytes_out = 4 * scan_ws_floats(B, L, D, N);
+  return TESM_OK;
+}
 
 extern "C" int tesm_b200_ssm_scan(const void *x, const void *dt, const void *bm, const void *cm, const void *z,
                                   void *out, const int64_t *strides, int dtype, int64_t B, int64_t L, int64_t D,
                                   int64_t N, const float *A, const float *skip, const float *dt_bias, int softplus,
-                                  float *state, const int32_t *lengths, tesm_stream_t stream) {
+                                  float *state, const int32_t *lengths, void *ws, int64_t ws_bytes, tesm_stream_t stream) {
   using namespace tesm;
   if (dtype != TESM_F32 && dtype != TESM_BF16) return fail(TESM_EDTYPE, "ssm_scan: dtype");
-  TESM_REQUIRE(B >= 0 && L >= 0 && D >= 0 && L < (1ll << 30) && D < (1ll << 30), "ssm_scan: bad shape");
+  TESM_REQUIRE(scan_shape_ok(B, L, D), "ssm_scan: bad shape");
   if (N < 1 || N > 128) return fail(TESM_EUNSUPPORTED, "ssm_scan: 1 to 128 states per channel");
   if (B == 0 || L == 0 || D == 0) return TESM_OK;
   TESM_REQUIRE(x && dt && bm && cm && out && A && strides, "ssm_scan: null pointer");
-  TESM_REQUIRE(B * ceil_div(D, 4) < (1ll << 31), "ssm_scan: too many blocks");
   const int64_t es = dtype == TESM_BF16 ? 2 : 4, *ld = strides;
   for (int i = 0; i < 12; ++i) TESM_REQUIRE(ld[i] >= 0, "ssm_scan: negative stride");
   TESM_REQUIRE(!self_overlap(B, L, D, ld[10], ld[11]), "ssm_scan: out overlaps itself");
+  const int64_t need = 4 * scan_ws_floats(B, L, D, N);
+  TESM_REQUIRE(need == 0 || (ws && ws_bytes >= need && ((uintptr_t)ws & 15) == 0), "ssm_scan: workspace");
   const Span so = span3(out, B, L, D, ld[10], ld[11], es), ss = span1(state, B * D * N * 4);
+  const Span sw = need ? span1(ws, need) : Span{};
   for (const Span &r : {span3(x, B, L, D, ld[0], ld[1], es), span3(dt, B, L, D, ld[2], ld[3], es),
                         span3(bm, B, L, N, ld[4], ld[5], es), span3(cm, B, L, N, ld[6], ld[7], es),
                         span3(z, B, L, D, ld[8], ld[9], es), span1(A, D * N * 4), span1(skip, D * 4),
                         span1(dt_bias, D * 4), span1(lengths, B * 4)})
-    TESM_REQUIRE(!so.meets(r) && !ss.meets(r), "ssm_scan: out or state shares memory with an input");
-  TESM_REQUIRE(!so.meets(ss), "ssm_scan: out shares memory with state");
+    TESM_REQUIRE(!so.meets(r) && !ss.meets(r) && !sw.meets(r), "ssm_scan: out, state or workspace shares memory with an input");
+  TESM_REQUIRE(!so.meets(ss) && !so.meets(sw) && !ss.meets(sw), "ssm_scan: out, state and workspace share memory");
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == TESM_BF16) {
     ScanArgs<__nv_bfloat16> a = {};
     a.A = A, a.skip = skip, a.dt_bias = dt_bias, a.state = state, a.lengths = lengths;
     a.L = (int)L, a.D = (int)D, a.N = (int)N, a.softplus = softplus;
-    return ssm_scan_c<__nv_bfloat16>(x, dt, bm, cm, z, out, strides, B, a, st);
+    return ssm_scan_c<__nv_bfloat16>(x, dt, bm, cm, z, out, strides, B, a, (float *)ws, st);
   }
   ScanArgs<float> a = {};
   a.A = A, a.skip = skip, a.dt_bias = dt_bias, a.state = state, a.lengths = lengths;
   a.L = (int)L, a.D = (int)D, a.N = (int)N, a.softplus = softplus;
-  return ssm_scan_c<float>(x, dt, bm, cm, z, out, strides, B, a, st);
+  return ssm_scan_c<float>(x, dt, bm, cm, z, out, strides, B, a, (float *)ws, st);
 }

@@ -740,6 +740,13 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     return out
 
 
+@lru_cache(maxsize=256)
+def _scan_workspace(B: int, L: int, D: int, N: int) -> int:
+    n = ctypes.c_int64(0)
+    _lib.call("tesm_b200_ssm_scan_workspace", B, L, D, N, ctypes.addressof(n))
+    return n.value
+
+
 def ssm_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, Bm: torch.Tensor, Cm: torch.Tensor, *,
              D: Optional[torch.Tensor] = None, z: Optional[torch.Tensor] = None,
              dt_bias: Optional[torch.Tensor] = None, softplus: bool = True, state: Optional[torch.Tensor] = None,
@@ -775,7 +782,9 @@ def ssm_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, Bm: torch.Tenso
     _check(what, "state", state, (B, C, N), torch.float32, dev)
     _check(what, "lengths", lengths, (B,), torch.int32, dev)
     _no_grad(what, x, dt, A, Bm, Cm, D, z, dt_bias, state)
+    ws_bytes = _scan_workspace(B, L, C, N) if L > 1 else 0
+    ws = A.new_empty(ws_bytes // 4) if ws_bytes else None
     _call_on(dev, "tesm_b200_ssm_scan", x.data_ptr(), dt.data_ptr(), Bm.data_ptr(), Cm.data_ptr(), _ptr(z),
              out.data_ptr(), strides, code, B, L, C, N, A.data_ptr(), _ptr(D), _ptr(dt_bias), softplus, _ptr(state),
-             _ptr(lengths))
+             _ptr(lengths), _ptr(ws), ws_bytes)
     return out

@@ -88,17 +88,37 @@ def test_conv_refuses(kw, want):
     assert conv(**kw) == want
 
 
-def scan(dtype=0, B=1, L=4, D=8, N=16, x=P, A=P, out=P, strides=True):
+def scan(dtype=0, B=1, L=4, D=8, N=16, x=P, A=P, out=P, strides=True, ws=None, ws_bytes=0):
     s = (ctypes.c_int64 * 12)(*[64] * 12)
     return status("tesm_b200_ssm_scan", x, P, P, P, None, out, ctypes.addressof(s) if strides else None, dtype, B, L, D, N,
-                  A, None, None, 1, None, None, None)
+                  A, None, None, 1, None, None, ws, ws_bytes, None)
 
 
-@pytest.mark.parametrize("kw,want", [(dict(dtype=3), 2), (dict(B=-1), 1), (dict(L=1 << 30), 1), (dict(N=0), 5),
+@pytest.mark.parametrize("kw,want", [(dict(dtype=3), 2), (dict(B=-1), 1), (dict(B=1 << 62), 1), (dict(L=1 << 30), 1), (dict(N=0), 5),
                                      (dict(N=129), 5), (dict(x=None), 1), (dict(A=None), 1), (dict(out=None), 1),
                                      (dict(strides=False), 1), (dict(B=1 << 29, D=64), 1), (dict(L=0), 0), (dict(D=0), 0)])
 def test_scan_refuses(kw, want):
     assert scan(**kw) == want
+
+
+def test_scan_workspace():
+    """Long sequences of few channels need one; the call checks it before anything else runs."""
+    n = ctypes.c_int64(-1)
+    assert status("tesm_b200_ssm_scan_workspace", 1, 4096, 64, 16, ctypes.addressof(n)) == 0 and n.value > 0
+    need = n.value
+    for shape in [(1, 1, 64, 16), (1, 100, 64, 16), (0, 4096, 64, 16), (1, 4096, 0, 16), (64, 4096, 8192, 16)]:
+        assert status("tesm_b200_ssm_scan_workspace", *shape, ctypes.addressof(n)) == 0 and n.value == 0
+    assert status("tesm_b200_ssm_scan_workspace", 1, 4096, 64, 129, ctypes.addressof(n)) == 1
+    assert status("tesm_b200_ssm_scan_workspace", 1, 4096, 64, 16, None) == 1
+    s = (ctypes.c_int64 * 12)(*[64 * 4096, 64, 64 * 4096, 64, 16 * 4096, 16, 16 * 4096, 16, 0, 0, 64 * 4096, 64])
+    at = [ctypes.c_void_p((i + 1) << 30) for i in range(8)]
+    for ws, size in [(None, need), (at[6], need - 1), (ctypes.c_void_p((7 << 30) + 8), need)]:
+        assert status("tesm_b200_ssm_scan", at[0], at[1], at[2], at[3], None, at[4], ctypes.addressof(s), 0, 1, 4096, 64, 16,
+                      at[5], None, None, 1, None, None, ws, size, None) == 1
+        assert "workspace" in _lib.last_error()
+    for i in range(6):  # a workspace inside an input, A or out
+        assert status("tesm_b200_ssm_scan", at[0], at[1], at[2], at[3], None, at[4], ctypes.addressof(s), 0, 1, 4096, 64, 16,
+                      at[5], None, None, 1, None, None, at[i], need, None) == 1
 
 
 def test_rows_disjoint():
@@ -156,7 +176,8 @@ def test_scan_refuses_shared_memory(which, written):
         at[written] = at[which] + 4
     t = (ctypes.c_int64 * 12)(*s)
     assert status("tesm_b200_ssm_scan", *(vp(at[n]) for n in ("x", "dt", "bm", "cm", "z", "out")), ctypes.addressof(t), 0, 2, 4,
-                  8, 16, vp(at["A"]), vp(at["skip"]), vp(at["bias"]), 1, vp(at["state"]), vp(at["lengths"]), None) == 1
+                  8, 16, vp(at["A"]), vp(at["skip"]), vp(at["bias"]), 1, vp(at["state"]), vp(at["lengths"]), None, 0,
+                  None) == 1
 
 
 def test_cpu_tensors_are_refused():
