@@ -695,11 +695,14 @@ static int pad_states(int64_t N) {
 // cutting the sequences wins (8192 tokens, 2048 channels, 16 states: 544 us whole, 281 in 4, 248 in 8, 219
 // in 16 segments; 512 tokens: 22 in 4, 29 whole).  At 7 warps per 8 schedulers it is about even (4096
 // channels: 119 us in 16 segments, 108 whole at 2048 tokens, 227 and 266 at 4096, whose inputs
-// leave L2) and above it loses (8192 channels: 341 us whole, 402 in 2).  Segments have 128 tokens at
-// least, and under four of them do not pay for the second launch.
+// leave L2) and above it loses (8192 channels: 341 us whole, 402 in 2).  16 segments, or up to 32 while
+// they fit the SMs at once (8192 tokens, 2048 channels of one state: 123 us in 32, 173 in 16; with 16
+// states 241 and 218).  Segments have 128 tokens at least, and under four of them do not pay for the
+// second launch.
 static int64_t scan_segment(int64_t B, int64_t L, int64_t D, int64_t N) {
-  const int64_t warps = ceil_div(B * D * (int64_t)pad_states(N), 128);
-  const int64_t s = L / 128 < 16 ? L / 128 : 16;
+  const int64_t warps = ceil_div(B * D * (int64_t)pad_states(N), 128);  // B, D > 0
+  const int64_t fill = 16 * (int64_t)sm_count() / warps, most = fill < 16 ? 16 : fill > 32 ? 32 : fill;
+  const int64_t s = L / 128 < most ? L / 128 : most;
   return s < 4 || 2 * warps > 7 * (int64_t)sm_count() ? L : round_up(ceil_div(L, s), kScanAhead);
 }
 static int64_t scan_ws_floats(int64_t B, int64_t L, int64_t D, int64_t N) {
