@@ -327,6 +327,12 @@ struct ScanShape {
   static constexpr int BLOCKS = NP > 16 ? 2 : 4;    // per SM that the registers allow: 16 states, 4 sequences: 506 us, with 2 blocks 631
 };
 
+// A in powers of two; an infinite one times a step of 0, as behind the end, is 0 and not NaN.
+__device__ __forceinline__ float rate2(float A) {
+  A *= kLog2e;
+  return isinf(A) ? copysignf(3.4e38f, A) : A;
+}
+
 // h 2^e for the e of a whole segment.  Token by token a state that is 0 or infinite stays so, and one
 // that underflows or overflows halfway to its value does not exist: hence four steps, each of which
 // stays in range where the result does.
@@ -360,8 +366,7 @@ __global__ void __launch_bounds__(kScanThreads, ScanShape<NPT, LPC>::BLOCKS) k_s
 #pragma unroll
   for (int i = 0; i < NPT; ++i) {
     const bool on = live && n0 + i < a.N;
-    const float A = on ? a.A[(int64_t)c * a.N + n0 + i] * kLog2e : 0.f;
-    A2[i] = isinf(A) ? copysignf(3.4e38f, A) : A;  // times the 0 of a token behind the end: 0, not NaN
+    A2[i] = on ? rate2(a.A[(int64_t)c * a.N + n0 + i]) : 0.f;
     h[i] = 0.f;
     if (!on) continue;
     if constexpr (ENDS) {
@@ -546,7 +551,7 @@ __global__ void __launch_bounds__(kStepThreads, 5) k_ssm_step(const __grid_const
   Pack<float, 4> A;
   load4(A, a.A + (int64_t)c * a.N + n0, true);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) A.v[i] *= kLog2e;
+  for (int i = 0; i < 4; ++i) A.v[i] = rate2(A.v[i]);
   const float bias = live && a.dt_bias ? a.dt_bias[c] : 0.f, skip = live && a.skip ? a.skip[c] : 0.f;
   const int64_t row = (int64_t)a.D * a.N;
   float *st = a.state ? a.state + b0 * row + (int64_t)c * a.N + n0 : nullptr;

@@ -324,18 +324,24 @@ def test_scan_in_segments_growth(first):
     check_scan(kw)
 
 
-def test_scan_infinite_A():
+@pytest.mark.parametrize("lengths", [(9, 4), (1, 1)])
+def test_scan_infinite_A(lengths):
     """A = -inf forgets at every token, and only there: not at the padding behind the end."""
-    kw = inputs(26, 2, 9, 5, 4, torch.float32)
+    L = max(lengths)
+    kw = inputs(26, 2, L, 5, 4, torch.float32)
     kw["A"][:] = float("-inf")
     a = cuda(kw)
     ops.ssm_scan(a["x"], a["dt"], a["A"], a["Bm"], a["Cm"], dt_bias=a["dt_bias"], state=a["state"],
-                 lengths=torch.tensor([9, 4], dtype=torch.int32, device="cuda"))
-    for b, n in enumerate((9, 4)):
+                 lengths=torch.tensor(lengths, dtype=torch.int32, device="cuda"))
+    for b, n in enumerate(lengths):
         dt = torch.nn.functional.softplus(kw["dt"][b, n - 1].double() + kw["dt_bias"].double())
         h = (dt * kw["x"][b, n - 1].double())[:, None] * kw["Bm"][b, n - 1].double()
         # softplus as in scan64: (1 + |raw| (2^-3 + 2^-4)) 2^-20 with |raw| < 8, two products
         assert ((a["state"][b].cpu().double() - h).abs() <= h.abs() * 3 * 2.0 ** -20).all()
+    a["dt"].zero_()
+    before = a["state"].clone()
+    ops.ssm_scan(a["x"], a["dt"], a["A"], a["Bm"], a["Cm"], softplus=False, state=a["state"])
+    assert torch.equal(a["state"], before)
 
 
 def test_scan_in_segments_captured():
