@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(kConvThreads)
 // partial sums exchange halves in log2(LPC) rounds), which gates and stores it.  So the
 // per-channel work is done once, and only B and C, shared by all channels, go through shared
 // memory, in fp32 tiles of 64 tokens.
-// One bf16 sequence of 4096 tokens, 8192 channels, 16 states: 340 us.  Neither its bytes bound it
+// One bf16 sequence of 4096 tokens, 8192 channels, 16 states: 334 us.  Neither its bytes bound it
 // (41 us) nor its 20 exponentials and reciprocals per token and channel (149 us at 16 a clock and
 // SM), but the 9 instructions per state, at 0.4 of the issue rate with the 7 warps that an SM
 // gets from one sequence; four sequences of 2048 tokens, twice the work, take 506 us.  Inputs staged
@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(kScanThreads, ScanShape<NPT, LPC>::BLOCKS) k_s
 #pragma unroll
   for (int i = 0; i < NPT; ++i) {
     const bool on = live && n0 + i < a.N;
-    A2[i] = on ? rate2(a.A[(int64_t)c * a.N + n0 + i]) : 0.f;
+    A2[i] = rate2(on ? a.A[(int64_t)c * a.N + n0 + i] : 0.f);
     h[i] = 0.f;
     if (!on) continue;
     if constexpr (ENDS) {
