@@ -435,6 +435,12 @@ static int beam_splits(int64_t R, int64_t V, int dtype) {
   return s < 1 ? 1 : (int)s;
 }
 
+// Sizes of which no product leaves 64 bits and no grid 31.
+static bool beam_shape_ok(int64_t G, int64_t W, int64_t V, int64_t K) {
+  return W >= 1 && W <= kMaxBeams && K >= 1 && K <= kMaxBeams && V >= 1 && V <= (1ll << 30) && G >= 0 &&
+         G <= ((1ll << 24) - 1) / W;
+}
+
 static int64_t beam_ws_bytes(int64_t R, int64_t K, int64_t S) { return R * S * (int64_t)(sizeof(RowStat) + K * 8); }
 
 // ------------------------------------------------------------ states follow their beams
@@ -520,8 +526,7 @@ extern "C" int tesm_b200_beam_select_workspace(int dtype, int64_t G, int64_t W, 
   using namespace tesm;
   if (dtype != TESM_F32 && dtype != TESM_BF16) return fail(TESM_EDTYPE, "beam_select_workspace: dtype");
   TESM_REQUIRE(bytes_out, "beam_select_workspace: null pointer");
-  TESM_REQUIRE(G >= 0 && V >= 1 && W >= 1 && W <= kMaxBeams && K >= 1 && K <= kMaxBeams,
-               "beam_select_workspace: bad shape");
+  TESM_REQUIRE(beam_shape_ok(G, W, V, K), "beam_select_workspace: bad shape");
   *bytes_out = G ? beam_ws_bytes(G * W, K, beam_splits(G * W, V, dtype)) : 0;
   return TESM_OK;
 }
@@ -533,9 +538,8 @@ extern "C" int tesm_b200_beam_select(const void *logits, int dtype, int64_t ldg,
                                      int32_t *out_lengths, void *ws, int64_t ws_bytes, tesm_stream_t stream) {
   using namespace tesm;
   if (dtype != TESM_F32 && dtype != TESM_BF16) return fail(TESM_EDTYPE, "beam_select: dtype");
-  TESM_REQUIRE(G >= 0 && W >= 1 && W <= kMaxBeams && K >= 1 && K <= kMaxBeams,
-               "beam_select: 1 to 32 beams in and out");
-  TESM_REQUIRE(V >= 1 && V <= (1ll << 30) && G * W < (1ll << 24), "beam_select: bad shape");
+  TESM_REQUIRE(W >= 1 && W <= kMaxBeams && K >= 1 && K <= kMaxBeams, "beam_select: 1 to 32 beams in and out");
+  TESM_REQUIRE(beam_shape_ok(G, W, V, K), "beam_select: bad shape");
   TESM_REQUIRE(pad >= 0 && pad < (1ll << 31), "beam_select: bad pad token");
   TESM_REQUIRE(length_penalty == length_penalty && (length_penalty == 0.0 || lengths),
                "beam_select: a length penalty needs lengths");

@@ -1,0 +1,32 @@
+"""Serving operators at the limits of their entry points: sizes whose products leave 64 bits, and what
+the checks on the host let through.  Without a GPU."""
+import ctypes
+
+import pytest
+
+from tesm_b200 import _lib
+
+P = ctypes.c_void_p(1 << 20)  # never dereferenced: the checks come first
+
+
+def status(name, *args):
+    return getattr(_lib.load(), name)(*args)
+
+
+@pytest.mark.parametrize("G,W", [(1 << 62, 4), (1 << 59, 32), (1 << 60, 16), ((1 << 62) + 1, 4), (1 << 24, 1),
+                                 (((1 << 24) - 1) // 3 + 1, 3)])
+def test_beam_prompts_whose_rows_leave_64_bits(G, W):
+    """A product G * W that wraps to 0 would divide by 0, which ends the process: refused instead."""
+    n = ctypes.c_int64(-1)
+    assert status("tesm_b200_beam_select_workspace", 0, G, W, 100, 4, ctypes.addressof(n)) == 1 and n.value == -1
+    assert status("tesm_b200_beam_select", P, 0, 400, 100, G, W, 100, 4, P, None, None, -1, 0, 0.0, P, P, P, P, P, P, 1 << 30,
+                  None) == 1
+    assert "bad shape" in _lib.last_error()
+
+
+def test_beam_prompts_up_to_the_limit():
+    n = ctypes.c_int64(-1)
+    for W in (1, 3, 32):
+        assert status("tesm_b200_beam_select_workspace", 1, ((1 << 24) - 1) // W, W, 1 << 30, 32, ctypes.addressof(n)) == 0
+        assert n.value > 0
+    assert status("tesm_b200_beam_select_workspace", 1, 1, 1, (1 << 30) + 1, 32, ctypes.addressof(n)) == 1
