@@ -800,11 +800,13 @@ extern "C" int tesm_b200_causal_conv(const void *x, int dtype, int64_t ldxb, int
                                      tesm_stream_t stream) {
   using namespace tesm;
   if (dtype != TESM_F32 && dtype != TESM_BF16) return fail(TESM_EDTYPE, "causal_conv: dtype");
-  TESM_REQUIRE(B >= 0 && L >= 0 && D >= 0 && L < (1ll << 30) && D < (1ll << 30), "causal_conv: bad shape");
+  TESM_REQUIRE(B >= 0 && L >= 0 && D >= 0 && B < (1ll << 31) && L < (1ll << 30) && D < (1ll << 30),
+               "causal_conv: bad shape");
   if (K < 2 || K > 8) return fail(TESM_EUNSUPPORTED, "causal_conv: kernel width 2 to 8");
   if (B == 0 || L == 0 || D == 0) return TESM_OK;
   TESM_REQUIRE(x && weight && out, "causal_conv: null pointer");
-  TESM_REQUIRE(B * ceil_div(D, kConvThreads) * ceil_div(L, 8) < (1ll << 31), "causal_conv: too many blocks");
+  const int64_t chunks = ceil_div(D, kConvThreads);  // products below 2^54 and, behind the first check, 2^58
+  TESM_REQUIRE(B * chunks < (1ll << 31) && B * chunks * ceil_div(L, 8) < (1ll << 31), "causal_conv: too many blocks");
   const int64_t es = dtype == TESM_BF16 ? 2 : 4;
   TESM_REQUIRE(ldxb >= 0 && ldxl >= 0 && ldob >= 0 && ldol >= 0, "causal_conv: negative stride");
   TESM_REQUIRE(!self_overlap(B, L, D, ldob, ldol), "causal_conv: out overlaps itself");

@@ -30,3 +30,12 @@ def test_beam_prompts_up_to_the_limit():
         assert status("tesm_b200_beam_select_workspace", 1, ((1 << 24) - 1) // W, W, 1 << 30, 32, ctypes.addressof(n)) == 0
         assert n.value > 0
     assert status("tesm_b200_beam_select_workspace", 1, 1, 1, (1 << 30) + 1, 32, ctypes.addressof(n)) == 1
+
+
+@pytest.mark.parametrize("B,L,D", [((1 << 62) + 1, 1, 512), (1 << 62, 1, 512), ((1 << 40) + 1, 1 << 29, 1 << 29), (1 << 31, 1, 1),
+                                   ((1 << 30) + 1, 1 << 29, 1 << 29)])
+def test_conv_sequences_whose_blocks_leave_64_bits(B, L, D):
+    """The number of blocks wraps to a small one, and (int)B with it: only a part would be computed."""
+    x, w, out = (ctypes.c_void_p(1 << k) for k in (41, 43, 45))
+    assert status("tesm_b200_causal_conv", x, 0, 0, 0, B, L, D, 4, w, None, None, None, 1, out, D, 0, None) == 1
+    assert "bad shape" in _lib.last_error() or "blocks" in _lib.last_error()
