@@ -65,10 +65,25 @@ struct alignas(N * sizeof(T) >= 16 ? 16 : N * sizeof(T)) Pack {
       if (vec && have >= N) {
 #pragma unroll
         for (int i = 0; i < (int)(N * sizeof(T) / 16); ++i)
+          reinterpret_cast<uint4 *>(v)[i] = reinterpret_cast<const uint4 *>(p)[i];
+        return;
+      }
+    }
+    load_single(p, have);
+  }
+  // for memory that the kernel does not write
+  __device__ __forceinline__ void load_read_only(const T *p, bool vec, int have) {
+    if constexpr (N * sizeof(T) % 16 == 0) {
+      if (vec && have >= N) {
+#pragma unroll
+        for (int i = 0; i < (int)(N * sizeof(T) / 16); ++i)
           reinterpret_cast<uint4 *>(v)[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
         return;
       }
     }
+    load_single(p, have);
+  }
+  __device__ __forceinline__ void load_single(const T *p, int have) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = i < have ? p[i] : from_f<T>(0.f);
   }
@@ -185,10 +200,10 @@ __global__ void __launch_bounds__(kConvThreads)
   for (int b = b0; b < b1; ++b) {
     const int T_b = seq_len(lengths, b, L), te = min(t1, T_b);
     T *st = state ? state + (int64_t)b * (K - 1) * D + c : nullptr;
-    // the input of position p >= 1 - K; before the start the state's rows
+    // the input of position p >= 1 - K; before the start the state's rows, which this kernel replaces
     auto load = [&](Pack<T, N> &q, int p) {
       if (p >= 0)
-        q.load(x.at(b, p, c), vec, have);
+        q.load_read_only(x.at(b, p, c), vec, have);
       else if (st)
         q.load(st + (int64_t)(p + K - 1) * D, vec, have);
       else
@@ -208,7 +223,7 @@ __global__ void __launch_bounds__(kConvThreads)
             const uint32_t at = (uint32_t)(t + u - t0) % (kGroups * U) * (kConvThreads * 16);
             if (t + u < te) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot + at), "l"(xp) : "memory");
           } else {
-            next[u].load(xp, vec, t + u < te ? have : 0);
+            next[u].load_read_only(xp, vec, t + u < te ? have : 0);
           }
           xp += x.ldl;
         }
@@ -404,8 +419,8 @@ __global__ void __launch_bounds__(kScanThreads, ScanShape<NPT, LPC>::BLOCKS) k_s
     for (int i = 0; i < BIPT; ++i) {
       const int it = tid + i * kScanThreads, t = t0 + it / (NP / BV), n = it % (NP / BV) * BV;
       const int have = it < S::BITEMS && t < T_b ? a.N - n : 0;
-      nb[i].load(a.bm.at(b, t, n), a.vec_bc, have);
-      if constexpr (!ENDS) nc[i].load(a.cm.at(b, t, n), a.vec_bc, have);
+      nb[i].load_read_only(a.bm.at(b, t, n), a.vec_bc, have);
+      if constexpr (!ENDS) nc[i].load_read_only(a.cm.at(b, t, n), a.vec_bc, have);
     }
   };
 #pragma unroll

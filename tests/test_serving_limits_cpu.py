@@ -1,6 +1,8 @@
 """Serving operators at the limits of their entry points: sizes whose products leave 64 bits, and what
 the checks on the host let through.  Without a GPU."""
 import ctypes
+import pathlib
+import re
 
 import pytest
 
@@ -39,3 +41,15 @@ def test_conv_sequences_whose_blocks_leave_64_bits(B, L, D):
     x, w, out = (ctypes.c_void_p(1 << k) for k in (41, 43, 45))
     assert status("tesm_b200_causal_conv", x, 0, 0, 0, B, L, D, 4, w, None, None, None, 1, out, D, 0, None) == 1
     assert "bad shape" in _lib.last_error() or "blocks" in _lib.last_error()
+
+
+def test_memory_that_a_kernel_writes_is_not_read_through_the_read_only_path():
+    """``__ldg`` is defined for memory that nobody writes while the kernel runs; the convolution shifts its
+    window of inputs in place, so the window's rows come through ordinary loads."""
+    text = (pathlib.Path(__file__).parents[1] / "tesm_b200" / "csrc" / "ssm.cu").read_text()
+    pack = text[text.index("struct alignas"):text.index("\n};", text.index("struct alignas"))]
+    bodies = re.split(r"__device__ __forceinline__ void (?=\w+\()", pack)[1:]
+    read_only = [b.split("(")[0] for b in bodies if "__ldg" in b]
+    assert read_only, "the test no longer finds the loads"
+    calls = re.findall(r"\.(\w+)\((?:st|state|a\.state|ahead)\b", text)
+    assert "load" in calls and not set(calls) & set(read_only), (calls, read_only)
