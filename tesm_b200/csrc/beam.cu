@@ -310,10 +310,11 @@ __global__ void __launch_bounds__(kRowThreads, kRowBlocks)
 // the parts' lists its K best logits.  Keys are formed in fp64, so that two candidates of a row
 // whose log-probabilities round to the same fp32 keep the order of their logits; the logarithms and
 // powers of all beams are taken by one warp, lane per beam, since fp64 functions cost as much for
-// one lane as for 32.  Launched while the first kernel runs; it waits for it where it reads its output.
+// one lane as for 32.  Launched while the first kernel runs; it waits for it where it reads its output,
+// which is not __restrict__: as constant for this kernel's life it could be loaded before the wait.
 __global__ void __launch_bounds__(1024)
-    k_beam_pick(const RowStat *__restrict__ stat, const float *__restrict__ cval, const int *__restrict__ cidx, int W,
-                int V, int K, int S, const float *__restrict__ scores, const uint8_t *__restrict__ finished,
+    k_beam_pick(const RowStat *stat, const float *cval, const int *cidx, int W, int V, int K, int S,
+                const float *__restrict__ scores, const uint8_t *__restrict__ finished,
                 const int *__restrict__ lengths, int64_t eos, int64_t pad, double alpha,
                 int64_t *__restrict__ tokens, int *__restrict__ parents, float *__restrict__ out_scores,
                 uint8_t *__restrict__ out_finished, int *__restrict__ out_lengths) {

@@ -53,3 +53,15 @@ def test_memory_that_a_kernel_writes_is_not_read_through_the_read_only_path():
     assert read_only, "the test no longer finds the loads"
     calls = re.findall(r"\.(\w+)\((?:st|state|a\.state|ahead)\b", text)
     assert "load" in calls and not set(calls) & set(read_only), (calls, read_only)
+
+
+def test_memory_written_while_a_kernel_waits_is_not_declared_read_only():
+    """The selection's second kernel is resident while the first writes its statistics and lists: declared
+    const __restrict__ they would count as constant for the kernel's life, and the compiler could load
+    them before the wait."""
+    text = (pathlib.Path(__file__).parents[1] / "tesm_b200" / "csrc" / "beam.cu").read_text()
+    head = re.search(r"k_beam_pick\((.*?)\) \{", text, re.S).group(1)
+    params = [" ".join(p.split()) for p in head.split(",")]
+    for name in ("stat", "cval", "cidx"):
+        (p,) = [p for p in params if re.search(rf"\b{name}$", p)]
+        assert "*" in p and "__restrict__" not in p, p
