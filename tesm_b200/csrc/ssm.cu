@@ -2,6 +2,8 @@
 // single tokens.
 #include "common.cuh"
 
+#include <numeric>
+
 namespace tesm {
 
 // x * sigmoid(x); 0 for x -> -inf (the reciprocal of inf is 0, and x * 0 stays finite for finite x)
@@ -131,15 +133,28 @@ __device__ __forceinline__ int seq_len(const int *lengths, int64_t b, int L) {
 // ------------------------------------------------------------ host-side checks of what is written
 struct Span {
   uintptr_t lo, hi;
-  bool meets(const Span &o) const { return lo < o.hi && o.lo < hi; }
+  uintptr_t row, pitch;  // bytes of a row; rows lie at lo plus multiples of pitch (0: one row)
+  // Columns of one buffer, as slices of a projection, lie between one another without a shared byte: so
+  // it is where the rows, modulo the distance that all of them keep, do not meet.
+  bool meets(const Span &o) const {
+    if (lo >= o.hi || o.lo >= hi) return false;
+    if (o.lo < lo) return o.meets(*this);
+    const uintptr_t g = std::gcd(pitch, o.pitch);
+    if (g == 0) return true;
+    const uintptr_t off = (o.lo - lo) % g;
+    return off < row || off + o.row > g;
+  }
 };
-// bytes of a (B, L, n) tensor of `es`-byte elements with element strides ldb, ldl
+// a (B, L, n) tensor of `es`-byte elements with element strides ldb, ldl
 static Span span3(const void *p, int64_t B, int64_t L, int64_t n, int64_t ldb, int64_t ldl, int64_t es) {
-  if (!p) return Span{0, 0};
+  if (!p) return Span{};
   const uintptr_t lo = (uintptr_t)p;
-  return Span{lo, lo + (uintptr_t)(((B - 1) * ldb + (L - 1) * ldl + n) * es)};
+  return Span{lo, lo + (uintptr_t)(((B - 1) * ldb + (L - 1) * ldl + n) * es), (uintptr_t)(n * es),
+              (uintptr_t)(std::gcd(B > 1 ? ldb : 0, L > 1 ? ldl : 0) * es)};
 }
-static Span span1(const void *p, int64_t bytes) { return p ? Span{(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes} : Span{0, 0}; }
+static Span span1(const void *p, int64_t bytes) {
+  return p ? Span{(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes, (uintptr_t)bytes, 0} : Span{};
+}
 // whether a (B, L, n) tensor holds an element twice
 static bool self_overlap(int64_t B, int64_t L, int64_t n, int64_t ldb, int64_t ldl) {
   if (B > 1 && L > 1)

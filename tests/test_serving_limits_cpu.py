@@ -5,6 +5,7 @@ import pathlib
 import re
 
 import pytest
+import torch
 
 from tesm_b200 import _lib
 
@@ -65,3 +66,39 @@ def test_memory_written_while_a_kernel_waits_is_not_declared_read_only():
     for name in ("stat", "cval", "cidx"):
         (p,) = [p for p in params if re.search(rf"\b{name}$", p)]
         assert "*" in p and "__restrict__" not in p, p
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="what the checks let through must find no device to run on")
+def test_shared_memory_by_brute_force():
+    """x and out (2, 3, n) float32 at strides and distances drawn at random: refused wherever a byte is
+    shared, and let through as columns of one buffer."""
+    g = torch.Generator().manual_seed(1)
+    r = lambda lo, hi: int(torch.randint(lo, hi, (1,), generator=g))  # noqa: E731
+    w = ctypes.c_void_p(1 << 40)
+    passed = interleaved = 0
+    for i in range(3000):
+        n, base = r(1, 5), 1 << 20
+        shape = [(r(1, 4), r(1, 4), n)] * 2
+        if i % 2:  # columns of one buffer
+            wide = 2 * n + r(0, 4)
+            ld = [(wide * shape[0][1], wide) if i % 4 == 1 else (wide, wide * shape[0][0])] * 2
+        else:
+            ld = [(r(0, 40), r(0, 16)) for _ in range(2)]
+        off = r(-12, 60)
+        x, out = (set(4 * (o + b * lb + t * lt + c) + k for b in range(B) for t in range(T) for c in range(n) for k in range(4))
+                  for (B, T, n), (lb, lt), o in zip(shape, ld, (0, off)))
+        B, T, _ = shape[0]
+        rc = status("tesm_b200_causal_conv", ctypes.c_void_p(base), 0, *ld[0], B, T, n, 2, w, None, None, None, 1,
+                    ctypes.c_void_p(base + 4 * off), *ld[1], None)
+        assert rc in (1, 3)
+        if x & out or len(out) < 4 * B * T * n:
+            assert rc == 1, (shape, ld, off)
+        elif i % 2:
+            # the rows as a whole lie apart, or between one another without a common byte modulo the buffer's width
+            at = off % wide if off >= 0 else wide - (-off) % wide
+            between = n <= at and at + n <= wide
+            apart = max(x) < min(out) or max(out) < min(x)
+            assert rc == 3 or not (between or apart), (shape, ld, off)
+            interleaved += between and not apart
+        passed += rc == 3
+    assert passed > 300 and interleaved > 50
