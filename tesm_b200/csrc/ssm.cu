@@ -702,7 +702,7 @@ static int launch_scan_k(K kern, const A &a, int64_t blocks, int threads, int sm
 template <class T, int NPT, int LPC>
 static int launch_scan(ScanArgs<T> a, int64_t B, cudaStream_t st) {
   using S = ScanShape<NPT, LPC>;
-  a.chunks = (int)ceil_div(a.D, S::CT);
+  a.chunks = (int)ceil_div(a.D, S::CT);  // blocks as in scan_blocks
   if (a.segs > 1) {
     const int rc = launch_scan_k(k_ssm_scan<T, NPT, LPC, true>, a, B * a.chunks * (a.segs - 1), kScanThreads, S::SMEM, st);
     if (rc) return rc;
@@ -725,20 +725,38 @@ static int pad_states(int64_t N) {
   return np;
 }
 
+// Blocks of the prompt kernel, and how many of them an SM holds at once (as in ScanShape).
+static int64_t scan_blocks(int64_t B, int64_t D, int np) { return B * ceil_div(D, kScanThreads / (np > 4 ? np / 4 : 1)); }
+static int scan_resident(int np) { return np > 16 ? 2 : 4; }
+
 // Tokens per segment.  A warp's step takes about 65 ns however few warps there are, and 36 ns of its
-// scheduler where there are many; a second pass adds 22.  So with under one warp per scheduler
-// cutting the sequences wins (8192 tokens, 2048 channels, 16 states: 544 us whole, 281 in 4, 248 in 8, 219
-// in 16 segments; 512 tokens: 22 in 4, 29 whole).  At 7 warps per 8 schedulers it is about even (4096
-// channels: 119 us in 16 segments, 108 whole at 2048 tokens, 227 and 266 at 4096, whose inputs
-// leave L2) and above it loses (8192 channels: 341 us whole, 402 in 2).  16 segments, or up to 32 while
-// they fit the SMs at once (8192 tokens, 2048 channels of one state: 123 us in 32, 173 in 16; with 16
-// states 241 and 218).  Segments have 128 tokens at least, and under four of them do not pay for the
-// second launch.
+// scheduler where there are many; a second pass adds 22.  So with under one block (a warp per
+// scheduler) per SM cutting the sequences wins (8192 tokens, 2048 channels, 16 states: 544 us whole, 281
+// in 4, 248 in 8, 220 in 16 segments; 512 tokens: 22 in 4, 29 whole).  The most blocks per SM at which
+// it does, times 8, by sweeps of 1, 2, 4, ... 128 states over 0.12 to 3.5 blocks per SM and 512 to 8192
+// tokens, both types (time whole / time cut):
+//   1 state      18, from 4096 tokens on 20 (2.25: 1.04 to 1.11, 3: 0.86 to 0.94)
+//   2 states     14 (1.75: 1.2 to 1.3)
+//   4 to 16       7 (0.87: 16 states, 4096 tokens on 1.2 to 1.3; shorter ones 0.85 to 0.94 while their inputs
+//                 are in L2, 1.04 to 1.17 from memory; more blocks: 8192 channels 334 us whole, 402 in 2)
+//   above 16      4 below 4096 tokens (0.5: 1.1 to 1.5, 0.6: 0.9 to 1.16, 0.87: 0.6 to 0.8), 5 and from 8192 on
+//                 6 else (0.75 at 8192: 0.9 to 1.2)
+// Segments: as many as fit the SMs at once, up to 32, and 16 at least where they need not all fit: a
+// few whole rounds of short segments lose little.  At 2 blocks an SM and under 4096 tokens they do
+// (64 states, 0.25 blocks per SM, 2048 tokens: 40 us in 8, 49 in 16, 90 whole).  Segments have 128
+// tokens at least, and under four of them do not pay for the second launch.
 static int64_t scan_segment(int64_t B, int64_t L, int64_t D, int64_t N) {
-  const int64_t warps = ceil_div(B * D * (int64_t)pad_states(N), 128);  // B, D > 0
-  const int64_t fill = 16 * (int64_t)sm_count() / warps, most = fill < 16 ? 16 : fill > 32 ? 32 : fill;
+  const int np = pad_states(N);
+  const int64_t sm = sm_count(), blocks = scan_blocks(B, D, np);  // B, D > 0
+  const int limit = np == 1   ? (L < 4096 ? 18 : 20)
+                    : np == 2 ? 14
+                    : np <= 16 ? 7
+                               : (L < 4096 ? 4 : L < 8192 ? 5 : 6);
+  if (8 * blocks > limit * sm) return L;
+  const bool fit = np > 16 && L < 4096;
+  const int64_t room = scan_resident(np) * sm / blocks, most = room > 32 ? 32 : !fit && room < 16 ? 16 : room;
   const int64_t s = L / 128 < most ? L / 128 : most;
-  return s < 4 || 2 * warps > 7 * (int64_t)sm_count() ? L : round_up(ceil_div(L, s), kScanAhead);
+  return s < 4 ? L : round_up(ceil_div(L, s), kScanAhead);
 }
 static int64_t scan_ws_floats(int64_t B, int64_t L, int64_t D, int64_t N) {
   if (B == 0 || D == 0 || L <= 1) return 0;

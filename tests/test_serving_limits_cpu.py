@@ -102,3 +102,25 @@ def test_shared_memory_by_brute_force():
             interleaved += between and not apart
         passed += rc == 3
     assert passed > 300 and interleaved > 50
+
+
+def segments(B, L, D, N):
+    """Into how many segments a scan is cut: the workspace holds the states at each one's start and all sums
+    of steps but the last."""
+    n = ctypes.c_int64(-1)
+    assert status("tesm_b200_ssm_scan_workspace", B, L, D, N, ctypes.addressof(n)) == 0
+    s, rest = divmod(n.value // 4 + B * D, B * D * (N + 1))
+    assert n.value == 0 or rest == 0
+    return s if n.value else 1
+
+
+@pytest.mark.parametrize("B,L,D,N,want", [
+    # a block holds 128 channels of up to 4 states, an SM 4 blocks: 3 blocks per SM are no few channels
+    (1, 4096, 3 * 148 * 128, 1, 1), (8, 4096, 8192, 1, 1), (1, 4096, 74 * 128, 1, 16), (1, 8192, 2048, 1, 32),
+    # above 16 states an SM holds 2 blocks
+    (1, 2048, 128 * 16, 32, 1), (1, 1024, 111 * 8, 64, 1), (1, 2048, 37 * 8, 64, 8), (1, 2048, 74 * 4, 128, 4),
+    (1, 4096, 18 * 4, 128, 16), (3, 777, 771, 24, 1),
+    # 4 to 16 states
+    (1, 8192, 2048, 16, 16), (1, 4096, 4096, 16, 16), (1, 8192, 8192, 16, 1), (1, 512, 2048, 16, 4), (1, 511, 2048, 16, 1)])
+def test_scan_is_cut_where_few_blocks_run(B, L, D, N, want):
+    assert segments(B, L, D, N) == want

@@ -49,3 +49,23 @@ def test_scan_into_other_columns_of_its_projection(L, dtype):
     assert all(torch.equal(c, before[n]) for n, c in cols.items() if n != "out")
     with pytest.raises(_lib.TesmError):
         ops.ssm_scan(cols["x"], cols["dt"], a["A"], cols["Bm"], cols["Cm"], out=proj[..., C:2 * C])
+
+
+# ------------------------------------------------------------------ both sides of the cut into segments
+def segments(B, L, C, N):
+    """As cut by the scan: its workspace holds the states at the segments' starts and all sums of steps but one."""
+    n = ops._scan_workspace(B, L, C, N) // 4
+    return (n + B * C) // (B * C * (N + 1)) if n else 1
+
+
+@pytest.mark.parametrize("L,dtype", [(512, torch.bfloat16), (700, torch.float32), (1100, torch.bfloat16)])
+@pytest.mark.parametrize("N", [1, 2, 16, 24])
+def test_scan_on_both_sides_of_the_cut(N, L, dtype):
+    """The most channels that are cut and the fewest that are not, by what the workspace says."""
+    lo, hi = 1, 1 << 17
+    assert segments(1, L, lo, N) > 1 and segments(1, L, hi, N) == 1
+    while hi - lo > 1:
+        mid = (lo + hi) // 2
+        lo, hi = (mid, hi) if segments(1, L, mid, N) > 1 else (lo, mid)
+    for C in (lo, hi):
+        check_scan(inputs(L + C, 1, L, C, N, dtype, gate=L == 700, skip=L != 700))
