@@ -338,7 +338,9 @@ int tesm_b200_siso_scan_noalloc(const void *proj, int dtype, int64_t ldp, int64_
  * lengths[w] + 1; a beam with finished[w] != 0 offers itself alone (token `pad`, its score and
  * length unchanged; its logits are not read).  The K candidates with the largest
  * score / max(length, 1)^length_penalty win, ties go to the lower beam, then the lower token.
- * Candidates are formed and compared in fp64.  Outputs (G x K): tokens, parents (the beam
+ * The logits decide among the tokens of a beam, keys in fp64 among beams; the logsumexp in them is a sum of
+ * fp32 exponentials, so beams whose keys differ by less than about 1e-6 may change places.
+ * Outputs (G x K): tokens, parents (the beam
  * a candidate continues), scores, finished (parent finished, or token == eos; pass eos = -1 for
  * none), lengths.  Candidates of score -inf or NaN never win: a slot k that no candidate is left
  * for gets parent min(k, W - 1), token pad, score -inf, finished.  A NaN logit counts as -inf, +inf
@@ -386,7 +388,9 @@ int tesm_b200_causal_conv(const void *x, int dtype, int64_t ldxb, int64_t ldxl, 
  * element strides (batch, token) of x, dt, bm, cm, z, out.  A (D, N), skip (D), dt_bias (D) fp32, the
  * last two nullable.  state (B, D, N) fp32, dense, nullable: the state before the first token
  * (zeros without it), replaced by the one after the last.  lengths as in tesm_b200_causal_conv.  out
- * must not overlap the inputs, nor state anything.  1 <= N <= 128; states and sums in fp32.  ws:
+ * must not overlap the inputs, nor state anything.  1 <= N <= 128; states and sums in fp32.  An infinite A counts
+ * as one of 3.4e38 / log2(e).  A step or an x that is infinite or NaN makes its channel's outputs and
+ * states from there on infinite or NaN, either one; other channels do not see it.  ws:
  * 16-byte aligned scratch of tesm_b200_ssm_scan_workspace bytes (0 for most shapes: long sequences of
  * few channels run in two launches), free again once the work has run on the stream. */
 int tesm_b200_ssm_scan(const void *x, const void *dt, const void *bm, const void *cm, const void *z, void *out,

@@ -72,8 +72,10 @@ __device__ __forceinline__ void word_exchange(unsigned &w, int o, bool low) {
 
 // ------------------------------------------------------------ rows: softmax statistics and best logits
 // Each block takes one part of one row.  The pass over the part keeps, per thread, a running maximum
-// and the sum of exponentials below it (fp32; joined in fp64), nothing else: within a row the
-// order of the log-probabilities is the order of the logits, and the K-th largest of the 256
+// and the sum of exponentials below it, nothing else.  The exponentials are the hardware's (2^-22 relative)
+// and a thread's sum is fp32, joined in fp64: a score is off by up to about 1e-6, which can turn
+// round beams that near, never tokens of one beam; fp64 exponentials would cost many times the pass.  Within a row
+// the order of the log-probabilities is the order of the logits, and the K-th largest of the 256
 // threads' maxima bounds the part's K-th best logit from below.  So only the threads whose
 // maximum reaches it (K of them, more with ties) hold candidates, and of their logits only the
 // steps whose own maximum reaches it are read again.  240 fp32 rows of 151936 logits, 32 best: 41 us
@@ -307,7 +309,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowBlocks)
 
 // ------------------------------------------------------------ pick: the best keys over a prompt's beams
 // One block per prompt, one warp per beam: the parts' statistics give the row's log-normaliser,
-// the parts' lists its K best logits.  Keys are formed in fp64, so that two candidates of a row
+// the parts' lists its K best logits.  Keys are formed in fp64 from those statistics, so that two candidates of a row
 // whose log-probabilities round to the same fp32 keep the order of their logits; the logarithms and
 // powers of all beams are taken by one warp, lane per beam, since fp64 functions cost as much for
 // one lane as for 32.  Launched while the first kernel runs; it waits for it where it reads its output,

@@ -562,7 +562,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: Optional[int]
     logits (prompts, W, vocab) float32 or bfloat16 with unit vocabulary stride, scores (prompts, W)
     float32.  A live beam offers ``scores + log_softmax(logits)`` for every token, a ``finished`` one
     (bool) only itself with ``pad_token_id``; they are ranked by score / length ** length_penalty with
-    ``lengths`` (int32) counting the new token, ties to the lower beam, then the lower token.  Beams
+    ``lengths`` (int32) counting the new token, ties to the lower beam, then the lower token (beams
+    whose keys differ by less than about 1e-6 may change places: fp32 exponentials).  Beams
     start as ``scores = [0, -inf, ...]``: candidates of score -inf never win, and slots that
     nothing is left for come back finished with score -inf.  ``beams`` defaults to W; both at most 32."""
     what = "beam_select"
@@ -759,7 +760,9 @@ def ssm_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, Bm: torch.Tenso
     innermost stride, so slices of a projection are taken as they are; A (channels, N), D and dt_bias
     (channels,) float32; N = 1 .. 128.  ``state`` (B, channels, N) float32 holds h before the first token
     (zeros if not given) and is replaced by h after the last.  ``lengths`` (B,) int32: tokens of each
-    sequence (right-padded); outputs behind them are zeros and do not touch the state."""
+    sequence (right-padded); outputs behind them are zeros and do not touch the state.  A step or an x
+    that is infinite or NaN makes its channel's outputs and states from there on infinite or NaN; other
+    channels do not see it."""
     what = "ssm_scan"
     if x.dim() != 3 or not x.is_cuda:
         raise ValueError(f"tesm_b200 {what}: x must be a (batch, tokens, channels) CUDA tensor")
