@@ -168,7 +168,7 @@ static bool self_overlap(int64_t B, int64_t L, int64_t n, int64_t ldb, int64_t l
 // with the last K - 1 inputs in registers, two channels per packed FMA.  16 rows ahead are on
 // their way into the thread's own slots of shared memory: registers for as many would halve the
 // occupancy (4 rows ahead in registers: 116 us against 91 us, 5.9 TB/s, at 4 x 4096 tokens of 8192
-// bf16 channels, K = 4; a plain copy of the same bytes takes 87 us).  Rows are addressed by running
+// bf16 channels, K = 4, replayed from a graph; a plain copy of the same bytes takes 87 us).  Rows are addressed by running
 // pointers, since 64-bit products per row cost as much as the arithmetic.  Single tokens take kConvBatch
 // sequences per thread, so that the weights are read less often (256 sequences: 11 us, against 18 with one).
 constexpr int kConvThreads = 128, kConvBatch = 4;
@@ -338,7 +338,8 @@ struct ScanArgs {
 // -0.5), which a state adds up over as many tokens as it remembers.  2^2.9e-8 puts that back in the
 // FMA that forms the argument: mean error 2e-9 instead of -2e-8, states of 73 to 4000 tokens off by
 // 2e-7 to 6e-7 instead of 5e-7 to 15e-7 (relative norm; 6e-7 with expf).  A step of 0 still decays by
-// exactly 1, to which 2^2.9e-8 rounds.
+// exactly 1, to which 2^2.9e-8 rounds.  The bias is this chip's, found by measurement: on another it has to be
+// measured again.
 constexpr float kEx2Shift = 2.9e-8f;
 
 constexpr int kScanThreads = 128, kScanAhead = 32;
@@ -354,7 +355,9 @@ struct ScanShape {
   static constexpr int BITEMS = TT * (NP / BV);
   static constexpr int BIPT = (BITEMS + kScanThreads - 1) / kScanThreads;
   static constexpr int SMEM = 2 * TT * NP * 4;
-  static constexpr int BLOCKS = NP > 16 ? 2 : 4;    // per SM that the registers allow: 16 states, 4 sequences: 506 us, with 2 blocks 631
+  // Blocks per SM that the registers allow: 16 states, 4 sequences: 506 us, with 2 blocks 631.  Up to 8 states the
+  // rows ahead (PF) do not fit under that cap: 130 to 390 bytes a thread are spilled
+  static constexpr int BLOCKS = NP > 16 ? 2 : 4;
 };
 
 // A in powers of two; an infinite one times a step of 0, as behind the end, is 0 and not NaN.
@@ -555,7 +558,8 @@ __global__ void __launch_bounds__(kScanThreads, ScanShape<NPT, LPC>::BLOCKS) k_s
 // groups are on their way into the thread's own slots of shared memory, and the next group's
 // inputs into registers, while one group is computed.  256 sequences of 8192 bf16 channels, 16
 // states: 64 us, 4.4 TB/s; every lane forming softplus and gate for itself, one sequence at a time,
-// took 104 us, and 3 or 4 blocks of 256 threads per SM, which spill, 88 and 127 us.
+// took 104 us, and 3 or 4 blocks of 256 threads per SM, which spill, 88 and 127 us.  At the 5 blocks
+// that suit this case fp32 inputs spill about 100 bytes a thread (78 us; floor 46), unaligned bf16 ones 80.
 constexpr int kStepThreads = 128, kStepAhead = 2, kStepBatch = 16;
 
 template <class T, bool VEC, int LPC>
